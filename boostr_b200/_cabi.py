@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_int, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200q.so")
@@ -19,6 +19,15 @@ DT_F32, DT_BF16, DT_F16, DT_F64 = range(4)
 OP_QUANT_MATMUL, OP_QUANT_SWIGLU = 0, 1
 STATIC_SCRATCH_BYTES = 8 << 20
 TP_HANDLE_BYTES = 64
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("pages", c_size_t), ("page_size", c_size_t), ("kv_heads", c_size_t),
+                ("head_dim", c_size_t), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3)]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("row_stride", c_int64), ("head_stride", c_int64)]
+
 
 # every symbol include/b200q.h declares: name -> (restype, argtypes)
 SIGNATURES = {
@@ -57,6 +66,16 @@ SIGNATURES = {
     "b200q_col_parallel_matmul_gather": (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t,
                                                  c_int, c_int, POINTER(c_void_p), c_void_p]),
     "b200q_tp_all_reduce": (c_int, [c_void_p, c_size_t, c_int, c_int, POINTER(c_void_p), c_void_p]),
+    "b200q_paged_slots": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p, c_int64, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200q_rope_append": (c_int, [POINTER(Heads), POINTER(Heads), POINTER(Heads), c_int, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p,
+                                  c_size_t, c_size_t, c_int, c_void_p, c_void_p, c_float, POINTER(PagedCache), c_void_p, c_void_p, c_int,
+                                  c_void_p]),
+    "b200q_paged_decode_workspace_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t]),
+    "b200q_paged_decode": (c_int, [c_void_p, c_int, c_int64, c_int64, c_size_t, c_size_t, POINTER(PagedCache), c_void_p, c_int64, c_size_t,
+                                   c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "b200q_paged_prompt": (c_int, [c_void_p, c_int, c_int64, c_int64, c_size_t, c_size_t, c_void_p, c_size_t, POINTER(PagedCache), c_void_p,
+                                   c_int64, c_size_t, c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_int, c_void_p, c_void_p]),
     "b200q_launch_count": (ctypes.c_ulonglong, []),
 }
 

@@ -1,0 +1,276 @@
+"""Attention from a paged key-value cache: what stands between the q/k/v projections and the output projection.
+
+A serving step calls, in this order,
+
+* ``paged_slots``   once: the block tables, positions and cache slots of its new tokens, from the lengths of its requests;
+* ``rope_append``   in every layer: norms of each head's queries and keys, rotation by position, keys and values into the pages;
+* ``paged_decode``  attention of one new token per request, or ``paged_prompt`` of the new tokens of ragged prompts.
+
+A cache is two tensors [pages, page_size, kv_heads, head_dim] (bf16 or f16) of any strides whose last is 1, so a transposed
+[pages, kv_heads, page_size, head_dim] tensor and both halves of one tensor serve as well; ``new_cache`` makes one.  A block table
+[requests, width] (int32) names the pages of each request.  Lengths, tables and slots live on the GPU: nothing here waits for
+them, and all calls can be captured into a graph.  An index that is out of range is not followed;
+``ops.check_device_status`` reports it.
+
+Well-formed calls go through the compiled entry points of ``_hostops``; the Python form below takes the others and words the
+errors.  The calls enqueue on torch's current stream and do not synchronise.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _cabi
+from .format import QuantError
+from .ops import _DT, _out_buffer, _require_cuda, _stream, workspace
+
+
+class Slots(NamedTuple):
+    """The tables of a step (``paged_slots``)."""
+
+    block_table: torch.Tensor  # [requests, width] int32, the given one
+    seq_lens: torch.Tensor     # [requests] int32
+    cu_seqlens: torch.Tensor   # [requests + 1] int32
+    positions: torch.Tensor    # [tokens] int32
+    slots: torch.Tensor        # [tokens] int64
+    left: torch.Tensor         # [2] int32: pages left on the stack, pages that were missing
+
+
+def new_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda",
+              heads_first: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Zeroed keys and values [pages, page_size, kv_heads, head_dim]; ``heads_first``: the tokens of one head of a page are
+    neighbours in memory."""
+    shape = (pages, kv_heads, page_size, head_dim) if heads_first else (pages, page_size, kv_heads, head_dim)
+    k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+    return (k.transpose(1, 2), v.transpose(1, 2)) if heads_first else (k, v)
+
+
+def rope_tables(positions: int, rot: int, base: float = 10000.0, scaling: Optional[dict] = None, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin [positions, rot / 2] f32 of a rotation of ``rot`` elements, computed in 64 bits once.
+
+    ``scaling`` stretches the positions a model was trained on to longer contexts:
+
+    * ``{"type": "linear", "factor": f}``: every angle divided by f;
+    * ``{"type": "ntk", "factor": f}``: a larger base, so that the slowest angle is divided by f and the fastest kept;
+    * ``{"type": "llama3", "factor", "low_freq_factor", "high_freq_factor", "original_positions"}``: angles that turn fewer than
+      ``low`` times over the original positions divided by f, more than ``high`` times kept, a linear blend between;
+    * ``{"type": "yarn", "factor", "original_positions", "beta_fast", "beta_slow", "attention_factor"}``: the blend over the index
+      of the angle, and cos and sin scaled by the attention factor (0.1 ln f + 1 where it is not given)."""
+    if rot <= 0 or rot % 2 or positions <= 0:
+        raise QuantError(f"rope_tables: cannot rotate {rot} elements over {positions} positions")
+    s = dict(scaling or {"type": "none"})
+    kind, f, gain = s.get("type"), float(s.get("factor", 1.0)), 1.0
+    if not f > 0:
+        raise QuantError(f"rope_tables: factor must be positive, got {f}")
+    if kind == "ntk":
+        base = base * f ** (rot / (rot - 2)) if rot > 2 else base
+    inv = torch.tensor(float(base), dtype=torch.float64) ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    if kind == "linear":
+        inv = inv / f
+    elif kind == "llama3":
+        low, high, span = float(s["low_freq_factor"]), float(s["high_freq_factor"]), float(s["original_positions"])
+        keep = ((span * inv / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        inv = keep * inv + (1 - keep) * inv / f
+    elif kind == "yarn":
+        span = float(s["original_positions"])
+
+        def index(turns):  # where an angle turns that often over the original positions
+            return rot * math.log(span / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        first = max(math.floor(index(float(s.get("beta_fast", 32.0)))), 0)
+        last = min(math.ceil(index(float(s.get("beta_slow", 1.0)))), rot - 1)
+        keep = 1 - ((torch.arange(rot // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+        inv = keep * inv + (1 - keep) * inv / f
+        gain = float(s.get("attention_factor") or (0.1 * math.log(f) + 1.0 if f > 1 else 1.0))
+    elif kind not in ("none", "ntk"):
+        raise QuantError(f"rope_tables: unknown scaling '{kind}'")
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * inv
+    return (angle.cos() * gain).float().to(device), (angle.sin() * gain).float().to(device)
+
+
+def _ints(op: str, name: str, t: torch.Tensor, shape, dtype=torch.int32) -> torch.Tensor:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise QuantError(f"{op}: {name} must be {dtype} of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
+    _require_cuda(t, name)
+    return t.contiguous()
+
+
+def _table(op: str, t: torch.Tensor, requests: int) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != requests or t.shape[1] == 0:
+        raise QuantError(f"{op}: block_table must be torch.int32 of shape [{requests}, width], got {t.dtype} {list(t.shape)}")
+    _require_cuda(t, "block_table")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise QuantError(f"{op}: the rows of block_table must be contiguous")
+    return t
+
+
+def _cache(op: str, k: torch.Tensor, v: torch.Tensor) -> _cabi.PagedCache:
+    if k.dim() != 4 or tuple(k.shape) != tuple(v.shape) or k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+        raise QuantError(f"{op}: keys and values must be BF16 or F16 [pages, page_size, kv_heads, head_dim] alike, got {k.dtype} {list(k.shape)} "
+                         f"and {v.dtype} {list(v.shape)}")
+    _require_cuda(k, "k_cache")
+    _require_cuda(v, "v_cache")
+    if k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
+        raise QuantError(f"{op}: the elements of a head must be contiguous in the cache")
+    return _cabi.PagedCache(k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.shape[0], k.shape[1], k.shape[2], k.shape[3],
+                            (ctypes.c_int64 * 3)(*k.stride()[:3]), (ctypes.c_int64 * 3)(*v.stride()[:3]))
+
+
+def _same_device(op: str, first: torch.Tensor, *others) -> None:
+    if any(t is not None and t.device != first.device for t in others):
+        raise QuantError(f"{op}: all tensors must be on {first.device}")
+
+
+def paged_slots(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, page_size: int, free_pages: torch.Tensor,
+                free_count: torch.Tensor, tokens: int) -> Slots:
+    """The tables of a step in which request b, with ``ctx_lens[b]`` tokens in the cache, gets ``new_lens[b]`` more
+    (``b200q_paged_slots``).
+
+    The pages that the new tokens begin are taken from the stack ``free_pages[:free_count]`` (int32; the next one is the last) and
+    entered into ``block_table`` in place, -1 where the stack is empty.  ``tokens`` is the host's number of new tokens, or
+    a larger one that a graph was captured with: the rows behind the last token get position 0 and slot -1.
+    ``left[:1]`` is the next step's ``free_count``; ``left[1]`` is the number of pages that were missing."""
+    op = "paged_slots"
+    if ctx_lens.dim() != 1:
+        raise QuantError(f"{op}: ctx_lens must be 1D, got {list(ctx_lens.shape)}")
+    n = ctx_lens.shape[0]
+    ctx_lens, new_lens = _ints(op, "ctx_lens", ctx_lens, (n,)), _ints(op, "new_lens", new_lens, (n,))
+    free_count = _ints(op, "free_count", free_count, (1,))
+    free_pages = _ints(op, "free_pages", free_pages, (free_pages.numel(),))
+    _table(op, block_table, n)
+    _same_device(op, ctx_lens, new_lens, block_table, free_pages, free_count)
+    if tokens < 0 or page_size <= 0:
+        raise QuantError(f"{op}: bad page size {page_size} or {tokens} tokens")
+    i32 = dict(dtype=torch.int32, device=ctx_lens.device)
+    out = Slots(block_table, torch.empty(n, **i32), torch.empty(n + 1, **i32), torch.empty(tokens, **i32),
+                torch.empty(tokens, dtype=torch.int64, device=ctx_lens.device), torch.empty(2, **i32))
+    with torch.cuda.device(ctx_lens.device):
+        _cabi.check(_cabi.lib().b200q_paged_slots(
+            ctx_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], page_size,
+            free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), out.seq_lens.data_ptr(), out.cu_seqlens.data_ptr(),
+            out.positions.data_ptr(), out.slots.data_ptr(), tokens, out.left.data_ptr(), _stream()))
+    return out
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotated queries [tokens, q_heads, head_dim]; keys, rotated as well, and values go to ``slots`` of the cache, in one pass
+    (``b200q_rope_append``).
+
+    q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim] (F32, BF16 or F16): slices of one projection serve.
+    With ``q_weight`` / ``k_weight`` [head_dim] f32 each head is normalised first (RMSNorm).  The first 2 * cos.shape[1] elements
+    are rotated by the angles of ``positions`` (``rope_tables``): elements i and i + rot / 2 together, or 2i and 2i + 1
+    where ``interleaved``.  A negative slot: the token is not kept.  ``out_dtype``: q's type unless given."""
+    op = "rope_append"
+    cache = _cache(op, k_cache, v_cache)
+    d, hk = k_cache.shape[3], k_cache.shape[2]
+    out_dtype = out_dtype or (out.dtype if out is not None else q.dtype)
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise QuantError(f"{op}: q, k and v must be F32, BF16 or F16 alike, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if out_dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise QuantError(f"{op}: output must be F32, BF16 or F16, got {out_dtype}")
+    if q.dim() != 3 or q.shape[2] != d or tuple(k.shape) != (q.shape[0], hk, d) or tuple(v.shape) != tuple(k.shape):
+        raise QuantError(f"{op}: q, k and v must be [tokens, heads, {d}] with {hk} key-value heads, got {list(q.shape)}, {list(k.shape)} and "
+                         f"{list(v.shape)}")
+    t = q.shape[0]
+    _require_cuda(q, "q")
+    positions, slots = _ints(op, "positions", positions, (t,)), _ints(op, "slots", slots, (t,), torch.int64)
+    if cos.dim() != 2 or tuple(cos.shape) != tuple(sin.shape) or cos.dtype != torch.float32 or sin.dtype != torch.float32 or 2 * cos.shape[1] > d:
+        raise QuantError(f"{op}: cos and sin must be F32 [positions, rot / 2] with rot <= {d}, got {list(cos.shape)} and {list(sin.shape)}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (d,) or not w.is_cuda or not w.is_contiguous()):
+            raise QuantError(f"{op}: {name} must be a contiguous F32 CUDA tensor of {d} elements")
+    _same_device(op, q, k, v, positions, cos, sin, k_cache, v_cache, slots, q_weight, k_weight)
+    q, k, v = (x if x.stride(2) == 1 or d == 1 else x.contiguous() for x in (q, k, v))
+    cos, sin = cos.contiguous(), sin.contiguous()
+    out = _out_buffer(out, tuple(q.shape), out_dtype, q.device)
+    heads = [_cabi.Heads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (q, k, v)]
+    with torch.cuda.device(q.device):
+        _cabi.check(_cabi.lib().b200q_rope_append(
+            heads[0], heads[1], heads[2], _DT[q.dtype], t, q.shape[1], positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            2 * cos.shape[1], int(interleaved), None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), float(eps), cache, slots.data_ptr(), out.data_ptr(), _DT[out_dtype], _stream()))
+    return out
+
+
+def _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, out, out_dtype):
+    cache = _cache(op, k_cache, v_cache)
+    d, hk = k_cache.shape[3], k_cache.shape[2]
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % hk:
+        raise QuantError(f"{op}: queries must be [rows, q_heads, {d}] with a multiple of {hk} heads, got {list(q.shape)}")
+    if q.dtype not in (torch.float32, k_cache.dtype):
+        raise QuantError(f"{op}: queries must be F32 or of the cache's type {k_cache.dtype}, got {q.dtype}")
+    if seq_lens.dim() != 1:
+        raise QuantError(f"{op}: seq_lens must be 1D, got {list(seq_lens.shape)}")
+    if window < 0 or sinks < 0:
+        raise QuantError(f"{op}: window and sinks cannot be negative, got {window} and {sinks}")
+    _require_cuda(q, "q")
+    seq_lens = _ints(op, "seq_lens", seq_lens, seq_lens.shape)
+    _table(op, block_table, seq_lens.shape[0])
+    _same_device(op, q, k_cache, v_cache, block_table, seq_lens)
+    unit = 16 // q.element_size()
+    if (q.stride(2) != 1 and d > 1) or q.stride(0) % unit or q.stride(1) % unit:
+        q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out_dtype = out_dtype or (out.dtype if out is not None else q.dtype)
+    if out_dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise QuantError(f"{op}: output must be F32, BF16 or F16, got {out_dtype}")
+    out = _out_buffer(out, tuple(q.shape), out_dtype, q.device)
+    return cache, q, seq_lens, out, d ** -0.5 if scale is None else float(scale)
+
+
+def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 scale: Optional[float] = None, window: int = 0, sinks: int = 0, out_dtype: Optional[torch.dtype] = None,
+                 out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention of the newest token of each request over its pages (``b200q_paged_decode``).
+
+    q [requests, q_heads, head_dim], F32 or of the cache's type; ``seq_lens[b]`` tokens of request b are in the cache, the newest
+    among them.  ``scale`` is head_dim ** -0.5 unless given.  ``window`` > 0: the newest ``window`` tokens and the first ``sinks`` are
+    visible.  A request of length 0 (a padded row) gives zeros.  Returns out [requests, q_heads, head_dim], of q's type
+    unless ``out_dtype`` says otherwise, and with ``return_lse`` also the log-sum-exp of the scores [requests, q_heads] f32."""
+    op = "paged_decode"
+    cache, q, seq_lens, out, scale = _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, out, out_dtype)
+    n, hq, d = q.shape
+    if seq_lens.shape[0] != n:
+        raise QuantError(f"{op}: one row for each request: {n} rows and {seq_lens.shape[0]} lengths")
+    lse = torch.empty(n, hq, dtype=torch.float32, device=q.device) if return_lse else None
+    L = _cabi.lib()
+    with torch.cuda.device(q.device):
+        need = L.b200q_paged_decode_workspace_bytes(n, hq, d)
+        ws = workspace(need, q.device) if need else None
+        _cabi.check(L.b200q_paged_decode(q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), n, hq, cache, block_table.data_ptr(),
+                                         block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), scale, window, sinks, out.data_ptr(),
+                                         _DT[out.dtype], lse.data_ptr() if return_lse else None, ws.data_ptr() if need else None,
+                                         ws.numel() if need else 0, _stream()))
+    return (out, lse) if return_lse else out
+
+
+def paged_prompt(q: torch.Tensor, cu_seqlens: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                 seq_lens: torch.Tensor, scale: Optional[float] = None, window: int = 0, sinks: int = 0,
+                 out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Causal attention of the new tokens of ragged prompts, or of chunks of them, over their pages (``b200q_paged_prompt``).
+
+    q [tokens, q_heads, head_dim] of the cache's type: rows cu_seqlens[b] .. cu_seqlens[b + 1] are the newest of the ``seq_lens[b]``
+    tokens of request b, which are all in the cache.  Scale, window, sinks and results as in ``paged_decode``.  Rows of a
+    request of fewer tokens than rows, and rows behind the last request, are zero."""
+    op = "paged_prompt"
+    cache, q, seq_lens, out, scale = _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, out, out_dtype)
+    if q.dtype != k_cache.dtype:
+        raise QuantError(f"{op}: queries must be of the cache's type {k_cache.dtype}, got {q.dtype}")
+    t, hq, _ = q.shape
+    n = seq_lens.shape[0]
+    cu_seqlens = _ints(op, "cu_seqlens", cu_seqlens, (n + 1,))
+    _same_device(op, q, cu_seqlens)
+    lse = torch.empty(t, hq, dtype=torch.float32, device=q.device) if return_lse else None
+    with torch.cuda.device(q.device):
+        _cabi.check(_cabi.lib().b200q_paged_prompt(
+            q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), t, hq, cu_seqlens.data_ptr(), n, cache, block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), scale, window, sinks, out.data_ptr(), _DT[out.dtype],
+            lse.data_ptr() if return_lse else None, _stream()))
+    return (out, lse) if return_lse else out

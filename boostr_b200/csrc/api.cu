@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "../../include/b200q.h"
+#include "api.cuh"
 #include "common.cuh"
 #include "tmap.cuh"
 
@@ -289,6 +290,18 @@ int quant_matmul_impl(int format, const void* act, int act_dtype, const void* w,
 }
 
 }  // namespace
+
+namespace b200q {
+int api_fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(t_err, sizeof(t_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+unsigned int* api_status() { return status_ptr_current(); }
+int api_sm_count() { return sm_count_current(); }
+}  // namespace b200q
 
 extern "C" {
 
@@ -756,6 +769,7 @@ int b200q_check_device_status(void* stream) {
     if (e != cudaSuccess) return fail(B200Q_ERR_CUDA, "status read failed: %s", cudaGetErrorString(e));
     if (word) {
         cudaMemcpyToSymbol(g_status_word, &zero, sizeof(zero));
+        if (word == STATUS_BAD_INDEX) return fail(B200Q_ERR_INVALID_ARG, "a kernel met a page, slot, position or length out of range (status 0x%x)", word);
         return fail(B200Q_ERR_TIMEOUT, "a kernel gave up on a bounded wait (status 0x%x)", word);
     }
     return B200Q_OK;

@@ -1,0 +1,177 @@
+// C ABI of the operators around a paged key-value cache (declared in include/b200q.h): argument checks and launches.
+#include <cmath>
+
+#include "../../include/b200q.h"
+#include "api.cuh"
+#include "paged.cuh"
+
+namespace b200q {
+size_t slots_max_requests();
+cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st);
+cudaError_t launch_rope(const RopeParams& p, int dtype, bool interleaved, uint32_t run, cudaStream_t st);
+cudaError_t launch_attn_rows(const AttnParams& p, cudaStream_t st);
+}  // namespace b200q
+
+using namespace b200q;
+
+namespace {
+
+constexpr size_t MAX_INT = 0x7FFFFFFF;
+
+bool float_type(int t) { return t == DT_F32 || t == DT_BF16 || t == DT_F16; }
+size_t type_bytes(int t) { return t == DT_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int check_cache(const char* op, const b200q_paged_cache* c) {
+    if (!c || !c->k || !c->v) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null cache", op);
+    if (c->dtype != DT_BF16 && c->dtype != DT_F16) return api_fail(B200Q_ERR_UNSUPPORTED_DTYPE, "%s: the cache must be BF16 or F16, got dtype id %d", op, c->dtype);
+    if (c->pages == 0 || c->page_size == 0 || c->kv_heads == 0 || c->pages > MAX_INT || c->page_size > MAX_INT || c->kv_heads > 65535)
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: bad cache of %zu pages of %zu tokens and %zu heads", op, c->pages, c->page_size, c->kv_heads);
+    if (c->head_dim == 0 || c->head_dim % 8 || c->head_dim > 256)
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: head dimension must be a multiple of 8 up to 256, got %zu", op, c->head_dim);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: the cache must be 16-byte aligned", op);
+    for (int i = 0; i < 3; ++i)
+        if (c->k_strides[i] % 8 || c->v_strides[i] % 8 || c->k_strides[i] < 0 || c->v_strides[i] < 0)
+            return api_fail(B200Q_ERR_BAD_SHAPE, "%s: cache strides must be multiples of 8 elements", op);
+    return B200Q_OK;
+}
+
+int finish(const char* op, cudaError_t e) {
+    return e == cudaSuccess ? B200Q_OK : api_fail(B200Q_ERR_CUDA, "CUDA %s kernel launch failed: %s", op, cudaGetErrorString(e));
+}
+
+// What the two attentions share.
+int fill_attn(const char* op, AttnParams& p, const b200q_paged_cache* c, const void* q, int q_dtype, int64_t q_row, int64_t q_head, size_t rows,
+              size_t requests, size_t q_heads, const int32_t* table, int64_t table_row, size_t width, const int32_t* lens, float scale, size_t window,
+              size_t sinks, void* out, int out_dtype, float* lse) {
+    if (int rc = check_cache(op, c)) return rc;
+    if (!float_type(q_dtype) || !float_type(out_dtype)) return api_fail(B200Q_ERR_UNSUPPORTED_DTYPE, "%s: queries and output must be F32, BF16 or F16", op);
+    if (q_dtype != DT_F32 && q_dtype != c->dtype) return api_fail(B200Q_ERR_UNSUPPORTED_DTYPE, "%s: 16-bit queries must have the cache's type", op);
+    if (q_heads == 0 || q_heads % c->kv_heads || q_heads > 65535)
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: %zu query heads do not share %zu key-value heads evenly", op, q_heads, c->kv_heads);
+    if (rows > MAX_INT || requests > MAX_INT || width > MAX_INT || window > MAX_INT || sinks > MAX_INT || rows * q_heads > MAX_INT)
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: dimension too large (rows=%zu requests=%zu table width=%zu)", op, rows, requests, width);
+    if (!q || !table || !lens || !out) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
+    const int64_t unit = 16 / (int64_t)type_bytes(q_dtype);
+    if (!aligned(q, 16) || q_row % unit || q_head % unit || q_row < 0 || q_head < 0)
+        return api_fail(B200Q_ERR_INVALID_ARG, "%s: query heads must be 16-byte aligned", op);
+    if (!aligned(out, 16)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: output pointer must be 16-byte aligned", op);
+    if (width == 0 || table_row < 0) return api_fail(B200Q_ERR_BAD_SHAPE, "%s: empty block table", op);
+    if (!std::isfinite(scale)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: scale must be finite", op);
+    p.q = q, p.q_row = q_row, p.q_head = q_head, p.q_dtype = q_dtype;
+    p.k = static_cast<const uint8_t*>(c->k), p.v = static_cast<const uint8_t*>(c->v);
+    p.k_page = c->k_strides[0], p.k_tok = c->k_strides[1], p.k_head = c->k_strides[2];
+    p.v_page = c->v_strides[0], p.v_tok = c->v_strides[1], p.v_head = c->v_strides[2];
+    p.f16 = c->dtype == DT_F16;
+    p.table = table, p.table_row = table_row, p.width = (uint32_t)width, p.pages = (uint32_t)c->pages;
+    p.page.set((uint32_t)c->page_size);
+    p.lens = lens, p.cu = nullptr, p.rows = (uint32_t)rows, p.requests = (uint32_t)requests;
+    p.hq = (uint32_t)q_heads, p.hkv = (uint32_t)c->kv_heads, p.group = p.hq / p.hkv, p.dim = (uint32_t)c->head_dim;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.window = (uint32_t)window, p.sinks = (uint32_t)sinks;
+    p.out = out, p.out_dtype = out_dtype, p.lse = lse;
+    p.status = api_status();
+    if (!p.status) return api_fail(B200Q_ERR_CUDA, "%s: cannot resolve the device status word", op);
+    return B200Q_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200q_paged_slots(const int32_t* ctx_lens, const int32_t* new_lens, size_t requests, int32_t* block_table, int64_t table_row, size_t width,
+                      size_t page_size, const int32_t* free_pages, size_t free_capacity, const int32_t* free_count, int32_t* seq_lens,
+                      int32_t* cu_seqlens, int32_t* positions, int64_t* slots, size_t tokens, int32_t* left, void* stream) {
+    const char* op = "paged_slots";
+    if (requests == 0 || requests > slots_max_requests())
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: 1 to %zu requests, got %zu", op, slots_max_requests(), requests);
+    if (page_size == 0 || page_size > MAX_INT || width == 0 || width > MAX_INT || table_row < 0 || tokens > MAX_INT || free_capacity > MAX_INT)
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: bad page size %zu, table width %zu or %zu tokens", op, page_size, width, tokens);
+    if (!ctx_lens || !new_lens || !block_table || (!free_pages && free_capacity) || !free_count || !seq_lens || !cu_seqlens || !left ||
+        (tokens && (!positions || !slots)))
+        return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
+    SlotsParams p = {ctx_lens, new_lens, (uint32_t)requests, block_table, table_row, (uint32_t)width, {}, free_pages, free_count,
+                     (uint32_t)free_capacity, seq_lens, cu_seqlens, positions, slots, (uint32_t)tokens, left};
+    p.page.set((uint32_t)page_size);
+    return finish(op, launch_slots(p, api_sm_count(), static_cast<cudaStream_t>(stream)));
+}
+
+int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, const b200q_heads* v, int dtype, size_t tokens, size_t q_heads,
+                      const int32_t* positions, const float* cos, const float* sin, size_t table_rows, size_t rot, int interleaved,
+                      const float* q_weight, const float* k_weight, float eps, const b200q_paged_cache* cache, const int64_t* slots, void* out,
+                      int out_dtype, void* stream) {
+    const char* op = "rope_append";
+    if (int rc = check_cache(op, cache)) return rc;
+    if (!float_type(dtype) || !float_type(out_dtype)) return api_fail(B200Q_ERR_UNSUPPORTED_DTYPE, "%s: heads and output must be F32, BF16 or F16", op);
+    if (rot % 2 || rot > cache->head_dim) return api_fail(B200Q_ERR_BAD_SHAPE, "%s: %zu of %zu elements cannot be rotated", op, rot, cache->head_dim);
+    if (q_heads > 65535 || table_rows > MAX_INT || tokens > MAX_INT || tokens * (q_heads + 2 * cache->kv_heads) > MAX_INT)
+        return api_fail(B200Q_ERR_BAD_SHAPE, "%s: dimension too large (tokens=%zu heads=%zu)", op, tokens, q_heads);
+    if (tokens == 0) return B200Q_OK;
+    if (!q || !k || !v || !k->data || !v->data || (q_heads && (!q->data || !out)) || !positions || (rot && (!cos || !sin)) || !slots)
+        return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
+    const size_t in = type_bytes(dtype);
+    if (!aligned(q->data, in) || !aligned(k->data, in) || !aligned(v->data, in) || !aligned(out, type_bytes(out_dtype)))
+        return api_fail(B200Q_ERR_INVALID_ARG, "%s: heads must be aligned to their elements", op);
+    RopeParams p = {};
+    p.q = q->data, p.q_row = q->row_stride, p.q_head = q->head_stride;
+    p.k = k->data, p.k_row = k->row_stride, p.k_head = k->head_stride;
+    p.v = v->data, p.v_row = v->row_stride, p.v_head = v->head_stride;
+    p.tokens = (uint32_t)tokens, p.hq = (uint32_t)q_heads, p.hkv = (uint32_t)cache->kv_heads, p.dim = (uint32_t)cache->head_dim, p.rot = (uint32_t)rot;
+    p.heads.set(p.hq + 2 * p.hkv);
+    p.positions = positions, p.cos = cos, p.sin = sin, p.table_rows = rot ? (uint32_t)table_rows : 0xFFFFFFFFu;
+    p.q_weight = q_weight, p.k_weight = k_weight, p.eps = eps;
+    p.slots = slots, p.out = out, p.out_dtype = out_dtype;
+    p.k_cache = static_cast<uint8_t*>(cache->k), p.v_cache = static_cast<uint8_t*>(cache->v);
+    p.kc_page = cache->k_strides[0], p.kc_tok = cache->k_strides[1], p.kc_head = cache->k_strides[2];
+    p.vc_page = cache->v_strides[0], p.vc_tok = cache->v_strides[1], p.vc_head = cache->v_strides[2];
+    p.cache_dtype = cache->dtype, p.pages = (uint32_t)cache->pages;
+    p.page.set((uint32_t)cache->page_size);
+    p.status = api_status();
+    if (!p.status) return api_fail(B200Q_ERR_CUDA, "%s: cannot resolve the device status word", op);
+    // the longest run of elements that every row, both halves of the rotated part and its end are aligned to
+    uint32_t run = 8;
+    for (; run > 1; run /= 2) {
+        const int64_t r = run;
+        const size_t bi = in * run < 16 ? in * run : 16, bo = type_bytes(out_dtype) * run < 16 ? type_bytes(out_dtype) * run : 16;
+        if ((rot / 2) % run == 0 && p.q_row % r == 0 && p.q_head % r == 0 && p.k_row % r == 0 && p.k_head % r == 0 && p.v_row % r == 0 &&
+            p.v_head % r == 0 && aligned(p.q, bi) && aligned(p.k, bi) && aligned(p.v, bi) && aligned(p.out, bo))
+            break;
+    }
+    return finish(op, launch_rope(p, dtype, interleaved != 0, run, static_cast<cudaStream_t>(stream)));
+}
+
+size_t b200q_paged_decode_workspace_bytes(size_t requests, size_t q_heads, size_t head_dim) {
+    (void)requests, (void)q_heads, (void)head_dim;
+    return 0;
+}
+
+int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t requests, size_t q_heads,
+                       const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_row, size_t width, const int32_t* seq_lens,
+                       float scale, size_t window, size_t sinks, void* out, int out_dtype, float* lse, void* ws, size_t ws_bytes, void* stream) {
+    const char* op = "paged_decode";
+    if (requests == 0) return B200Q_OK;
+    AttnParams p = {};
+    if (int rc = fill_attn(op, p, cache, q, q_dtype, q_row_stride, q_head_stride, requests, requests, q_heads, block_table, table_row, width, seq_lens,
+                           scale, window, sinks, out, out_dtype, lse))
+        return rc;
+    (void)ws, (void)ws_bytes;
+    return finish(op, launch_attn_rows(p, static_cast<cudaStream_t>(stream)));
+}
+
+int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t tokens, size_t q_heads,
+                       const int32_t* cu_seqlens, size_t requests, const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_row,
+                       size_t width, const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out, int out_dtype, float* lse,
+                       void* stream) {
+    const char* op = "paged_prompt";
+    if (tokens == 0 || requests == 0) return B200Q_OK;
+    if (!cu_seqlens) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
+    if (q_dtype == DT_F32) return api_fail(B200Q_ERR_UNSUPPORTED_DTYPE, "%s: queries must have the cache's type", op);
+    AttnParams p = {};
+    if (int rc = fill_attn(op, p, cache, q, q_dtype, q_row_stride, q_head_stride, tokens, requests, q_heads, block_table, table_row, width, seq_lens,
+                           scale, window, sinks, out, out_dtype, lse))
+        return rc;
+    p.cu = cu_seqlens;
+    return finish(op, launch_attn_rows(p, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

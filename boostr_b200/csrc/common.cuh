@@ -18,8 +18,9 @@ enum : int { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2, DT_F64 = 3 };
 
 // Device status word (one per device, owned by the C-ABI translation unit and handed to
 // kernels as a pointer): a kernel that gives up on a bounded wait ORs a code in here and
-// finishes without touching the data it waited for.
-enum : unsigned { STATUS_TIMEOUT_FULL = 1u, STATUS_TIMEOUT_EMPTY = 2u, STATUS_TIMEOUT_MMA = 4u, STATUS_TIMEOUT_TMEM = 8u, STATUS_TIMEOUT_PEER = 16u };
+// finishes without touching the data it waited for.  BAD_INDEX: a page, slot, position or length read from device memory
+// was out of range and was not followed.
+enum : unsigned { STATUS_TIMEOUT_FULL = 1u, STATUS_TIMEOUT_EMPTY = 2u, STATUS_TIMEOUT_MMA = 4u, STATUS_TIMEOUT_TMEM = 8u, STATUS_TIMEOUT_PEER = 16u, STATUS_BAD_INDEX = 32u };
 
 __host__ __device__ constexpr int fmt_block_size(int f) { return (f == FMT_Q4_0 || f == FMT_Q5_0 || f == FMT_Q8_0) ? 32 : 256; }
 __host__ __device__ constexpr int fmt_block_bytes(int f) {

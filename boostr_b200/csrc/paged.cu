@@ -1,0 +1,297 @@
+// The bookkeeping and the writing side of a paged key-value cache: block tables and slot maps from request lengths, and the
+// norms, rotation and append of new queries, keys and values.
+#include "paged.cuh"
+
+namespace b200q {
+
+// ------------------------------------------------------------------------------------------------------------------ slots
+
+namespace {
+
+constexpr int SL_THREADS = 256;
+
+// Exclusive sum over the block; `total`: the sum over all threads.
+__device__ __forceinline__ uint2 block_scan(uint2 x, uint2& total) {
+    __shared__ uint2 part[SL_THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint2 s = x;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, s.x, d), b = __shfl_up_sync(0xFFFFFFFFu, s.y, d);
+        if (lane >= d) s.x += a, s.y += b;
+    }
+    if (lane == 31) part[warp] = s;
+    __syncthreads();
+    uint2 before = make_uint2(0, 0);
+    total = make_uint2(0, 0);
+#pragma unroll
+    for (int w = 0; w < SL_THREADS / 32; ++w) {
+        if (w == warp) before = total;
+        total.x += part[w].x;
+        total.y += part[w].y;
+    }
+    return make_uint2(before.x + s.x - x.x, before.y + s.y - x.y);
+}
+
+// Every block sums up all requests for itself (their number is small beside the cost of a second launch), keeps the running
+// sums of new tokens and new pages in shared memory, and serves its share of the tokens and of the new pages.  A token's
+// page is found from the sums, not from the table, which another block may be writing.
+__global__ void __launch_bounds__(SL_THREADS) slots_kernel(const SlotsParams p) {
+    extern __shared__ uint2 start[];  // [requests + 1] {first row, first new page} of each request
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t chunk = (p.requests + SL_THREADS - 1) / SL_THREADS;
+    const uint32_t b0 = min(p.requests, threadIdx.x * chunk), b1 = min(p.requests, b0 + chunk);
+    uint2 sum = make_uint2(0, 0);
+    uint32_t missing = 0;  // pages beyond the tables' width
+    for (uint32_t b = b0; b < b1; ++b) {
+        const uint32_t ctx = (uint32_t)max(p.ctx[b], 0), n = (uint32_t)max(p.fresh[b], 0);
+        const uint32_t held = p.page.div(ctx + p.page.d - 1), want = p.page.div(ctx + n + p.page.d - 1);
+        start[b] = sum;
+        sum.x += n;
+        sum.y += min(want, p.width) - min(held, p.width);
+        missing += want - held - (min(want, p.width) - min(held, p.width));
+    }
+    uint2 total;
+    const uint2 first = block_scan(sum, total);
+    for (uint32_t b = b0; b < b1; ++b) {
+        start[b].x += first.x;
+        start[b].y += first.y;
+    }
+    if (threadIdx.x == 0) start[p.requests] = total;
+    const uint32_t count = min((uint32_t)max(*p.free_count, 0), p.free_capacity);
+    const int any = __syncthreads_or((int)missing);
+    auto new_page = [&](uint32_t i) { return i < count ? p.free_pages[count - 1 - i] : -1; };
+    auto find = [&](uint32_t v, bool pages) {  // the last request that starts at or before v
+        uint32_t lo = 0, hi = p.requests;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if ((pages ? start[mid].y : start[mid].x) <= v) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    const uint32_t tid = blockIdx.x * SL_THREADS + threadIdx.x, nthreads = gridDim.x * SL_THREADS;
+    for (uint32_t i = tid; i < total.y; i += nthreads) {
+        const uint32_t b = find(i, true);
+        const uint32_t held = p.page.div((uint32_t)max(p.ctx[b], 0) + p.page.d - 1);
+        p.table[(int64_t)b * p.table_row + held + (i - start[b].y)] = new_page(i);
+    }
+    for (uint32_t t = tid; t < p.tokens; t += nthreads) {
+        int32_t pos = 0;
+        int64_t slot = -1;
+        if (t < total.x) {
+            const uint32_t b = find(t, false);
+            const uint32_t ctx = (uint32_t)max(p.ctx[b], 0);
+            const uint32_t at = ctx + (t - start[b].x), e = p.page.div(at), held = p.page.div(ctx + p.page.d - 1);
+            pos = (int32_t)at;
+            if (e < p.width) {
+                const int32_t page = e < held ? p.table[(int64_t)b * p.table_row + e] : new_page(start[b].y + (e - held));
+                if (page >= 0) slot = (int64_t)page * p.page.d + (at - e * p.page.d);
+            }
+        }
+        p.positions[t] = pos;
+        p.slots[t] = slot;
+    }
+    for (uint32_t b = tid; b <= p.requests; b += nthreads) {
+        p.cu[b] = (int32_t)start[b].x;
+        if (b < p.requests) p.seq_lens[b] = max(p.ctx[b], 0) + max(p.fresh[b], 0);
+    }
+    if (blockIdx.x == 0) {
+        // pages beyond the tables' width: rare, summed only when there are any
+        if (any) {
+            __shared__ uint32_t beyond;
+            if (threadIdx.x == 0) beyond = 0;
+            __syncthreads();
+            if (missing) atomicAdd(&beyond, missing);
+            __syncthreads();
+            missing = beyond;
+        }
+        if (threadIdx.x == 0) {
+            const uint32_t got = min(total.y, count);
+            p.left[0] = (int32_t)(count - got);
+            p.left[1] = (int32_t)(total.y - got + missing);
+        }
+    }
+}
+
+}  // namespace
+
+constexpr size_t SLOTS_MAX_REQUESTS = 16384;  // 128 KB of running sums in shared memory
+size_t slots_max_requests() { return SLOTS_MAX_REQUESTS; }
+
+cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st) {
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((SLOTS_MAX_REQUESTS + 1) * sizeof(uint2))); });
+    if (e != cudaSuccess) return e;
+    uint32_t blocks = (p.tokens + 4 * SL_THREADS - 1) / (4 * SL_THREADS);
+    blocks = blocks < 1 ? 1 : blocks > (uint32_t)sm_count ? (uint32_t)sm_count : blocks;
+    note_launch();
+    return launch_pdl(slots_kernel, dim3(blocks), dim3(SL_THREADS), (p.requests + 1) * sizeof(uint2), st, p);
+}
+
+// ------------------------------------------------------------------------------------------------------------------- rope
+
+namespace {
+
+constexpr int RP_THREADS = 256;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+// N consecutive elements as f32, in loads of up to 16 bytes
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float (&x)[2 * N], int at) {
+    constexpr int W = sizeof(T) * N > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+        const Pack<T, W> u = *reinterpret_cast<const Pack<T, W>*>(p + i);
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[at + i + j] = to_f32<T>(u.v[j]);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(void* base, int64_t i0, const float (&x)[2 * N], int at) {
+    constexpr int W = sizeof(T) * N > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+        Pack<T, W> u;
+#pragma unroll
+        for (int j = 0; j < W; ++j) u.v[j] = from_f32<T>(x[at + i + j]);
+        *reinterpret_cast<Pack<T, W>*>(static_cast<T*>(base) + i0 + i) = u;
+    }
+}
+
+// A row is one head of one token.  G neighbouring lanes share it; a lane owns U units of two runs of C elements: the two
+// that a rotation turns into one another (i and i + rot / 2 of the half layout; 2 C neighbours of the interleaved one), so
+// no element crosses lanes, or 2 C neighbours behind the rotated part.  Bound: HBM, each element is read and written once.
+template <typename T, int C, int G, int U, bool INTERLEAVED>
+__global__ void __launch_bounds__(RP_THREADS) rope_kernel(const RopeParams p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t row = blockIdx.x * (RP_THREADS / G) + threadIdx.x / G, g = threadIdx.x % G;
+    const bool live = row < p.tokens * p.heads.d;
+    const uint32_t t = live ? p.heads.div(row) : 0;
+    uint32_t h = live ? row - t * p.heads.d : 0;
+    const int kind = h < p.hq ? 0 : h < p.hq + p.hkv ? 1 : 2;  // query, key, value
+    if (kind) h -= kind == 1 ? p.hq : p.hq + p.hkv;
+    const T* src = kind == 0 ? static_cast<const T*>(p.q) + (int64_t)t * p.q_row + (int64_t)h * p.q_head
+                 : kind == 1 ? static_cast<const T*>(p.k) + (int64_t)t * p.k_row + (int64_t)h * p.k_head
+                             : static_cast<const T*>(p.v) + (int64_t)t * p.v_row + (int64_t)h * p.v_head;
+    const uint32_t half = p.rot / 2, turned = half / C;  // units that are turned
+    auto run = [&](uint32_t u, int j) {                   // first element of run j of unit u (>= dim: none)
+        return u < turned ? (INTERLEAVED ? 2 * C * u + C * j : C * u + half * j) : p.rot + 2 * C * (u - turned) + C * j;
+    };
+    float x[U][2 * C];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t e = run(g + G * i, j);
+            if (live && e < p.dim) load_n<T, C>(src + e, x[i], C * j);
+            else
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[i][C * j + c] = 0.f;
+        }
+    const float* w = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
+    if (p.q_weight || p.k_weight) {  // the same branch in every lane: the sums cross lanes
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int c = 0; c < 2 * C; ++c) s = fmaf(x[i][c], x[i][c], s);
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+        const float r = rsqrtf(s / (float)p.dim + p.eps);
+        if (w) {
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t e = run(g + G * i, j);
+                    if (e < p.dim)
+#pragma unroll
+                        for (int c = 0; c < C; ++c) x[i][C * j + c] *= r * __ldg(w + e + c);
+                }
+        }
+    }
+    if (!live) return;
+    if (kind < 2) {
+        const uint32_t pos = (uint32_t)p.positions[t];
+        if (pos >= p.table_rows) {  // no angle: nothing is written for this row
+            if (g == 0) atomicOr(p.status, STATUS_BAD_INDEX);
+            return;
+        }
+        const float *cs = p.cos + (int64_t)pos * half, *sn = p.sin + (int64_t)pos * half;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const uint32_t u = g + G * i;
+            if (u < turned)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float co = __ldg(cs + C * u + c), si = __ldg(sn + C * u + c);
+                    float &a = x[i][INTERLEAVED ? 2 * c : c], &b = x[i][INTERLEAVED ? 2 * c + 1 : C + c];
+                    const float a0 = a;
+                    a = a0 * co - b * si;
+                    b = b * co + a0 * si;
+                }
+        }
+    }
+    void* dst = p.out;
+    int64_t at = ((int64_t)t * p.hq + h) * p.dim;
+    int dtype = p.out_dtype;
+    if (kind) {
+        const int64_t slot = p.slots[t];
+        if (slot < 0) return;  // a token without a place in the cache
+        if (slot >= (int64_t)p.pages * p.page.d) {
+            if (g == 0) atomicOr(p.status, STATUS_BAD_INDEX);
+            return;
+        }
+        const int64_t page = slot < 0x7FFFFFFF ? (int64_t)p.page.div((uint32_t)slot) : slot / p.page.d, tok = slot - page * p.page.d;
+        dst = kind == 1 ? p.k_cache : p.v_cache;
+        at = kind == 1 ? page * p.kc_page + tok * p.kc_tok + (int64_t)h * p.kc_head : page * p.vc_page + tok * p.vc_tok + (int64_t)h * p.vc_head;
+        dtype = p.cache_dtype;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t e = run(g + G * i, j);
+            if (e < p.dim) {
+                if (dtype == DT_F32) store_n<float, C>(dst, at + e, x[i], C * j);
+                else if (dtype == DT_BF16) store_n<__nv_bfloat16, C>(dst, at + e, x[i], C * j);
+                else store_n<__half, C>(dst, at + e, x[i], C * j);
+            }
+        }
+}
+
+template <typename T, int C, int G, int U>
+cudaError_t rope_go(const RopeParams& p, bool interleaved, cudaStream_t st) {
+    const uint64_t rows = (uint64_t)p.tokens * p.heads.d, per = RP_THREADS / G;
+    const dim3 grid((unsigned)((rows + per - 1) / per));
+    note_launch();
+    return interleaved ? launch_pdl(rope_kernel<T, C, G, U, true>, grid, dim3(RP_THREADS), 0, st, p)
+                       : launch_pdl(rope_kernel<T, C, G, U, false>, grid, dim3(RP_THREADS), 0, st, p);
+}
+
+template <typename T>
+cudaError_t rope_typed(const RopeParams& p, bool interleaved, uint32_t run, cudaStream_t st) {
+    // runs of `run` elements are aligned and none crosses an end
+    if (run % 8 == 0) {
+        const uint32_t units = p.rot / 16 + (p.dim - p.rot + 15) / 16;
+        return units <= 8 ? rope_go<T, 8, 8, 1>(p, interleaved, st) : rope_go<T, 8, 16, 1>(p, interleaved, st);
+    }
+    if (run % 4 == 0) return rope_go<T, 4, 32, 1>(p, interleaved, st);
+    return rope_go<T, 1, 32, 4>(p, interleaved, st);
+}
+
+}  // namespace
+
+cudaError_t launch_rope(const RopeParams& p, int dtype, bool interleaved, uint32_t run, cudaStream_t st) {
+    return dtype == DT_F32 ? rope_typed<float>(p, interleaved, run, st)
+         : dtype == DT_BF16 ? rope_typed<__nv_bfloat16>(p, interleaved, run, st)
+                            : rope_typed<__half>(p, interleaved, run, st);
+}
+
+}  // namespace b200q

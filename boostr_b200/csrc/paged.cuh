@@ -1,0 +1,141 @@
+// What the kernels around the paged key-value cache share: the parameters of the two attentions, page look-up, 16-bit and
+// 32-bit element conversions.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200q {
+
+// n / d for 0 <= n < 2^31 by one multiplication: with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
+// floor(n / d) = (hi32(m n) + n) >> l (the round-up method of Granlund and Montgomery).
+struct FastDiv {
+    uint32_t d, m, l;
+    void set(uint32_t div) {
+        d = div;
+        for (l = 0; l < 32 && (1ull << l) < d;) ++l;
+        m = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> l; }
+};
+
+// Attention over a paged cache: rows of queries [rows, hq, dim] against the pages of their requests.  Strides in elements.
+struct AttnParams {
+    const void* q;
+    int64_t q_row, q_head;
+    int q_dtype;
+    const uint8_t *k, *v;              // bf16 or f16 elements
+    int64_t k_page, k_tok, k_head, v_page, v_tok, v_head;
+    bool f16;                          // element type of the cache
+    const int32_t* table;              // [requests, width], row stride table_row
+    int64_t table_row;
+    uint32_t width, pages;
+    FastDiv page;                      // tokens of a page
+    const int32_t* lens;               // [requests] tokens in the cache, the new ones among them
+    const int32_t* cu;                 // [requests + 1] first row of each request (nullptr: one row a request)
+    uint32_t rows, requests;
+    uint32_t hq, hkv, group, dim;
+    float scale_log2;                  // softmax scale times log2(e): weights are powers of two
+    uint32_t window, sinks;            // window 0: every key up to the row's own position
+    void* out;                         // [rows, hq, dim]
+    int out_dtype;
+    float* lse;                        // [rows, hq] or nullptr
+    unsigned int* status;
+};
+
+// Block tables, positions and slots of a step.
+struct SlotsParams {
+    const int32_t *ctx, *fresh;  // [requests] tokens in the cache, tokens of this step
+    uint32_t requests;
+    int32_t* table;              // [requests, width]
+    int64_t table_row;
+    uint32_t width;
+    FastDiv page;
+    const int32_t *free_pages, *free_count;  // a stack: the next page is free_pages[free_count - 1]
+    uint32_t free_capacity;
+    int32_t *seq_lens, *cu, *positions;
+    int64_t* slots;
+    uint32_t tokens;
+    int32_t* left;               // {pages left on the stack, pages that were missing}
+};
+
+// Norms, rotation and append of the new queries, keys and values.  Strides in elements.
+struct RopeParams {
+    const void *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    uint32_t tokens, hq, hkv, dim, rot;
+    FastDiv heads;                     // hq + 2 hkv
+    const int32_t* positions;
+    const float *cos, *sin;            // [table_rows, rot / 2]
+    uint32_t table_rows;
+    const float *q_weight, *k_weight;  // [dim] or nullptr
+    float eps;
+    const int64_t* slots;
+    void* out;                         // [tokens, hq, dim]
+    int out_dtype;
+    uint8_t *k_cache, *v_cache;
+    int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head;
+    int cache_dtype;
+    uint32_t pages;
+    FastDiv page;
+    unsigned int* status;
+};
+
+// Length of request b, within what its table can hold.
+__device__ __forceinline__ uint32_t attn_len(const AttnParams& p, uint32_t b) {
+    const int32_t n = p.lens[b];
+    const uint64_t most = (uint64_t)p.width * p.page.d;
+    if (n > 0 && (uint64_t)n > most) {
+        atomicOr(p.status, STATUS_BAD_INDEX);
+        return (uint32_t)most;
+    }
+    return n > 0 ? (uint32_t)n : 0u;
+}
+// Page of token j of request b; false (and the status word set): the table names none.
+__device__ __forceinline__ bool attn_page(const AttnParams& p, uint32_t b, uint32_t j, uint32_t& page, uint32_t& tok) {
+    const uint32_t e = p.page.div(j);
+    tok = j - e * p.page.d;
+    page = (uint32_t)p.table[(int64_t)b * p.table_row + e];
+    if (page < p.pages) return true;
+    atomicOr(p.status, STATUS_BAD_INDEX);
+    return false;
+}
+
+// Conversions between f32 and an element type (one rounding to nearest even).
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+__device__ __forceinline__ float load_f32(const void* p, int64_t i, int dtype) {
+    return dtype == DT_F32 ? static_cast<const float*>(p)[i] : dtype == DT_BF16 ? to_f32(static_cast<const __nv_bfloat16*>(p)[i]) : to_f32(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_f32(void* p, int64_t i, int dtype, float x) {
+    if (dtype == DT_F32) static_cast<float*>(p)[i] = x;
+    else if (dtype == DT_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+// The request whose rows hold row r: the last b with cu[b] <= r (cu[0] = 0; requests of no rows are passed over).
+__device__ __forceinline__ uint32_t request_of(const int32_t* cu, uint32_t requests, uint32_t r) {
+    uint32_t lo = 0, hi = requests;  // cu[lo] <= r < cu[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if ((uint32_t)cu[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+}  // namespace b200q

@@ -308,6 +308,87 @@ B200Q_API int b200q_col_parallel_matmul_gather(int format, const void* act, int 
  */
 B200Q_API int b200q_tp_all_reduce(void* data, size_t count, int rank, int world, void* const* bufs, void* stream);
 
+/*
+ * Attention from a paged key-value cache (decode and prompts), with the writing side of the cache.
+ *
+ * A cache is `pages` pages of `page_size` tokens; the keys and the values of head h of token t of page p begin at
+ * k + p * k_strides[0] + t * k_strides[1] + h * k_strides[2] (in elements; values likewise) and are head_dim consecutive
+ * elements.  So [page, token, head, dim] and [page, head, token, dim] memory, and keys and values in one tensor, are all
+ * served.  BF16 or F16; 16-byte aligned, strides multiples of 8 elements; head_dim a multiple of 8 up to 256.
+ * A block table names the pages of each request: row b, entry j holds tokens [j * page_size, (j + 1) * page_size).
+ *
+ * Unlike weights, everything here (tables, lengths, cache) is read in stream order.  A page, slot, position or length that
+ * is out of range is not followed; b200q_check_device_status then reports B200Q_ERR_INVALID_ARG, and the rows
+ * concerned are unspecified.
+ */
+typedef struct b200q_paged_cache {
+    void* k;
+    void* v;
+    int dtype; /* B200Q_BF16 or B200Q_F16 */
+    size_t pages, page_size, kv_heads, head_dim;
+    int64_t k_strides[3], v_strides[3]; /* page, token, head */
+} b200q_paged_cache;
+
+/* Heads of a batch of tokens: element e of head h of token t at data[t * row_stride + h * head_stride + e]. */
+typedef struct b200q_heads {
+    const void* data;
+    int64_t row_stride, head_stride; /* elements */
+} b200q_heads;
+
+/*
+ * The tables of a step: every request b, with ctx_lens[b] tokens in the cache, gets new_lens[b] more.
+ *   block_table [requests, width] (rows `table_row` elements apart): the pages that the new tokens begin are taken from the
+ *               stack free_pages[0 .. *free_count) (the next one is the last), in the order of the requests, and entered;
+ *               -1 where the stack is empty
+ *   seq_lens    [requests]     ctx_lens + new_lens
+ *   cu_seqlens  [requests + 1] running sum of new_lens: request b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1]
+ *   positions   [tokens]       position of each row in its request (0 behind the last row)
+ *   slots       [tokens]       page * page_size + offset of each row; -1 where it has no page, and behind the last row
+ *   left        [2]            pages left on the stack (the next *free_count), pages that were missing
+ * Lengths, the stack and the old entries are not changed, so `left` may go to the next step while this one runs.
+ * requests <= 16384.  Negative lengths count as 0.
+ */
+B200Q_API int b200q_paged_slots(const int32_t* ctx_lens, const int32_t* new_lens, size_t requests, int32_t* block_table, int64_t table_row,
+                                size_t width, size_t page_size, const int32_t* free_pages, size_t free_capacity, const int32_t* free_count,
+                                int32_t* seq_lens, int32_t* cu_seqlens, int32_t* positions, int64_t* slots, size_t tokens, int32_t* left,
+                                void* stream);
+
+/*
+ * Norms, rotation and append in one pass: q and k heads are normalised (RMSNorm over the head with q_weight / k_weight
+ * [head_dim] f32; NULL: not), their first `rot` elements rotated by the angles of their position (cos, sin [table_rows,
+ * rot / 2] f32), q is written to out [tokens, q_heads, head_dim], and k and v to slot slots[t] of the cache (negative: nowhere).
+ * interleaved: elements 2i and 2i + 1 are a pair; otherwise i and i + rot / 2.  One rounding, at the end.
+ * q, k, v of type `dtype` (F32, BF16 or F16), any strides; out may be q itself where the types agree and q is contiguous.
+ */
+B200Q_API int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, const b200q_heads* v, int dtype, size_t tokens, size_t q_heads,
+                                const int32_t* positions, const float* cos, const float* sin, size_t table_rows, size_t rot, int interleaved,
+                                const float* q_weight, const float* k_weight, float eps, const b200q_paged_cache* cache, const int64_t* slots,
+                                void* out, int out_dtype, void* stream);
+
+/*
+ * Attention of one new token per request, the last of its seq_lens[b] tokens (which is in the cache): out[b, h] =
+ * sum_j softmax_j(scale q[b, h] . k[j]) v[j] over the keys that it sees: all, or with window > 0 the last `window` and the
+ * first `sinks`.  A request of length 0 gives zeros (lse -inf).  q: F32 or the cache's type; out [requests, q_heads,
+ * head_dim] F32, BF16 or F16; lse [requests, q_heads] (natural logarithm of the sum of exponentials) or NULL.
+ * Scores, softmax and sums are f32; with F32 queries the products keep the queries' and weights' upper 16 bits or more.
+ */
+B200Q_API size_t b200q_paged_decode_workspace_bytes(size_t requests, size_t q_heads, size_t head_dim);
+B200Q_API int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t requests, size_t q_heads,
+                                 const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_row, size_t width,
+                                 const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out, int out_dtype, float* lse, void* ws,
+                                 size_t ws_bytes, void* stream);
+
+/*
+ * Causal attention of the new tokens of prompts, whole or in chunks: rows cu_seqlens[b] .. cu_seqlens[b + 1] of q are the
+ * last tokens of request b (all of which are in the cache), and each sees what a decode step at its position would.
+ * q of the cache's type.  Rows of a request that has more rows than tokens see nothing and are zero (lse -inf), and so are
+ * rows behind cu_seqlens[requests].
+ */
+B200Q_API int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t tokens, size_t q_heads,
+                                 const int32_t* cu_seqlens, size_t requests, const b200q_paged_cache* cache, const int32_t* block_table,
+                                 int64_t table_row, size_t width, const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out,
+                                 int out_dtype, float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

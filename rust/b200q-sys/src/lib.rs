@@ -38,6 +38,30 @@ pub const B200Q_OP_QUANT_SWIGLU: c_int = 1;
 pub const B200Q_STATIC_SCRATCH_BYTES: usize = 8 << 20;
 pub const B200Q_TP_HANDLE_BYTES: usize = 64;
 
+/// A paged key-value cache: `k + p * k_strides[0] + t * k_strides[1] + h * k_strides[2]` elements to head h of token t of page p.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct b200q_paged_cache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub dtype: c_int,
+    pub pages: usize,
+    pub page_size: usize,
+    pub kv_heads: usize,
+    pub head_dim: usize,
+    pub k_strides: [i64; 3],
+    pub v_strides: [i64; 3],
+}
+
+/// Heads of a batch of tokens; strides in elements.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct b200q_heads {
+    pub data: *const c_void,
+    pub row_stride: i64,
+    pub head_stride: i64,
+}
+
 #[link(name = "b200q")]
 extern "C" {
     pub fn b200q_version() -> c_int;
@@ -91,4 +115,21 @@ extern "C" {
                                             world: c_int, bufs: *const *mut c_void, stream: *mut c_void) -> c_int;
     pub fn b200q_tp_all_reduce(data: *mut c_void, count: usize, rank: c_int, world: c_int, bufs: *const *mut c_void,
                                stream: *mut c_void) -> c_int;
+    pub fn b200q_paged_slots(ctx_lens: *const i32, new_lens: *const i32, requests: usize, block_table: *mut i32, table_row: i64, width: usize,
+                             page_size: usize, free_pages: *const i32, free_capacity: usize, free_count: *const i32, seq_lens: *mut i32,
+                             cu_seqlens: *mut i32, positions: *mut i32, slots: *mut i64, tokens: usize, left: *mut i32,
+                             stream: *mut c_void) -> c_int;
+    pub fn b200q_rope_append(q: *const b200q_heads, k: *const b200q_heads, v: *const b200q_heads, dtype: c_int, tokens: usize, q_heads: usize,
+                             positions: *const i32, cos: *const f32, sin: *const f32, table_rows: usize, rot: usize, interleaved: c_int,
+                             q_weight: *const f32, k_weight: *const f32, eps: f32, cache: *const b200q_paged_cache, slots: *const i64,
+                             out: *mut c_void, out_dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn b200q_paged_decode_workspace_bytes(requests: usize, q_heads: usize, head_dim: usize) -> usize;
+    pub fn b200q_paged_decode(q: *const c_void, q_dtype: c_int, q_row_stride: i64, q_head_stride: i64, requests: usize, q_heads: usize,
+                              cache: *const b200q_paged_cache, block_table: *const i32, table_row: i64, width: usize, seq_lens: *const i32,
+                              scale: f32, window: usize, sinks: usize, out: *mut c_void, out_dtype: c_int, lse: *mut f32, ws: *mut c_void,
+                              ws_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn b200q_paged_prompt(q: *const c_void, q_dtype: c_int, q_row_stride: i64, q_head_stride: i64, tokens: usize, q_heads: usize,
+                              cu_seqlens: *const i32, requests: usize, cache: *const b200q_paged_cache, block_table: *const i32, table_row: i64,
+                              width: usize, seq_lens: *const i32, scale: f32, window: usize, sinks: usize, out: *mut c_void, out_dtype: c_int,
+                              lse: *mut f32, stream: *mut c_void) -> c_int;
 }
