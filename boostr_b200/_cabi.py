@@ -18,6 +18,7 @@ OK, ERR_INVALID_ARG, ERR_UNSUPPORTED_FORMAT, ERR_BAD_SHAPE, ERR_WORKSPACE_TOO_SM
 DT_F32, DT_BF16, DT_F16, DT_F64 = range(4)
 OP_QUANT_MATMUL, OP_QUANT_SWIGLU = 0, 1
 STATIC_SCRATCH_BYTES = 8 << 20
+PAGED_COUNTER_BYTES = 4096
 TP_HANDLE_BYTES = 64
 
 class PagedCache(ctypes.Structure):

@@ -25,7 +25,7 @@ import torch
 
 from . import _cabi
 from .format import QuantError
-from .ops import _DT, _out_buffer, _require_cuda, _stream, workspace
+from .ops import _DT, _out_buffer, _require_cuda, _stream
 
 
 class Slots(NamedTuple):
@@ -225,6 +225,24 @@ def _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, si
     return cache, q, seq_lens, out, d ** -0.5 if scale is None else float(scale)
 
 
+_decode_ws: dict = {}
+
+
+def _decode_workspace(nbytes: int, device) -> torch.Tensor:
+    """Scratch of ``paged_decode``, whose counters are zero between calls: one for each device and stream; a call that is being
+    captured gets one of its own, zeroed by the graph."""
+    nbytes = max(nbytes, 16)
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:_cabi.PAGED_COUNTER_BYTES].zero_()
+        return ws
+    key = (torch.device(device).index, torch.cuda.current_stream().cuda_stream)
+    ws = _decode_ws.get(key)
+    if ws is None or ws.numel() < nbytes:
+        _decode_ws[key] = ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return ws
+
+
 def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                  scale: Optional[float] = None, window: int = 0, sinks: int = 0, out_dtype: Optional[torch.dtype] = None,
                  out: Optional[torch.Tensor] = None, return_lse: bool = False):
@@ -242,12 +260,10 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     lse = torch.empty(n, hq, dtype=torch.float32, device=q.device) if return_lse else None
     L = _cabi.lib()
     with torch.cuda.device(q.device):
-        need = L.b200q_paged_decode_workspace_bytes(n, hq, d)
-        ws = workspace(need, q.device) if need else None
+        ws = _decode_workspace(L.b200q_paged_decode_workspace_bytes(hq, k_cache.shape[2], d), q.device)
         _cabi.check(L.b200q_paged_decode(q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), n, hq, cache, block_table.data_ptr(),
                                          block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), scale, window, sinks, out.data_ptr(),
-                                         _DT[out.dtype], lse.data_ptr() if return_lse else None, ws.data_ptr() if need else None,
-                                         ws.numel() if need else 0, _stream()))
+                                         _DT[out.dtype], lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), _stream()))
     return (out, lse) if return_lse else out
 
 

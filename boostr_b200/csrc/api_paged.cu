@@ -10,6 +10,8 @@ size_t slots_max_requests();
 cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st);
 cudaError_t launch_rope(const RopeParams& p, int dtype, bool interleaved, uint32_t run, cudaStream_t st);
 cudaError_t launch_attn_rows(const AttnParams& p, cudaStream_t st);
+size_t decode_workspace_bytes(uint32_t group, uint32_t dim, int sm_count);
+cudaError_t launch_decode(const AttnParams& p, void* ws, int sm_count, cudaStream_t st);
 }  // namespace b200q
 
 using namespace b200q;
@@ -140,9 +142,9 @@ int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, const b200q_he
     return finish(op, launch_rope(p, dtype, interleaved != 0, run, static_cast<cudaStream_t>(stream)));
 }
 
-size_t b200q_paged_decode_workspace_bytes(size_t requests, size_t q_heads, size_t head_dim) {
-    (void)requests, (void)q_heads, (void)head_dim;
-    return 0;
+size_t b200q_paged_decode_workspace_bytes(size_t q_heads, size_t kv_heads, size_t head_dim) {
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads || q_heads > 65535 || head_dim == 0 || head_dim > 256) return 0;
+    return decode_workspace_bytes((uint32_t)(q_heads / kv_heads), (uint32_t)head_dim, api_sm_count());
 }
 
 int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t requests, size_t q_heads,
@@ -154,8 +156,10 @@ int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_stride, int64_t
     if (int rc = fill_attn(op, p, cache, q, q_dtype, q_row_stride, q_head_stride, requests, requests, q_heads, block_table, table_row, width, seq_lens,
                            scale, window, sinks, out, out_dtype, lse))
         return rc;
-    (void)ws, (void)ws_bytes;
-    return finish(op, launch_attn_rows(p, static_cast<cudaStream_t>(stream)));
+    const size_t need = decode_workspace_bytes(p.group, p.dim, api_sm_count());
+    if (!ws || ws_bytes < need || !aligned(ws, 16))
+        return api_fail(B200Q_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes is too small or not 16-byte aligned, need %zu", op, ws ? ws_bytes : 0, need);
+    return finish(op, launch_decode(p, ws, api_sm_count(), static_cast<cudaStream_t>(stream)));
 }
 
 int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t tokens, size_t q_heads,

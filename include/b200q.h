@@ -370,9 +370,13 @@ B200Q_API int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, cons
  * sum_j softmax_j(scale q[b, h] . k[j]) v[j] over the keys that it sees: all, or with window > 0 the last `window` and the
  * first `sinks`.  A request of length 0 gives zeros (lse -inf).  q: F32 or the cache's type; out [requests, q_heads,
  * head_dim] F32, BF16 or F16; lse [requests, q_heads] (natural logarithm of the sum of exponentials) or NULL.
- * Scores, softmax and sums are f32; with F32 queries the products keep the queries' and weights' upper 16 bits or more.
+ * Scores, softmax and sums are f32; with F32 queries the products keep the queries' and weights' upper 16 bits or more
+ * (queries of an F16 cache below 65504).
+ * ws: b200q_paged_decode_workspace_bytes bytes (0: bad arguments), 16-byte aligned, whose first B200Q_PAGED_COUNTER_BYTES are zero before its first
+ * call; every call leaves them zero.  Calls that may overlap on the GPU must not share it.
  */
-B200Q_API size_t b200q_paged_decode_workspace_bytes(size_t requests, size_t q_heads, size_t head_dim);
+#define B200Q_PAGED_COUNTER_BYTES 4096
+B200Q_API size_t b200q_paged_decode_workspace_bytes(size_t q_heads, size_t kv_heads, size_t head_dim);
 B200Q_API int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t requests, size_t q_heads,
                                  const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_row, size_t width,
                                  const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out, int out_dtype, float* lse, void* ws,

@@ -123,7 +123,7 @@ extern "C" {
                              positions: *const i32, cos: *const f32, sin: *const f32, table_rows: usize, rot: usize, interleaved: c_int,
                              q_weight: *const f32, k_weight: *const f32, eps: f32, cache: *const b200q_paged_cache, slots: *const i64,
                              out: *mut c_void, out_dtype: c_int, stream: *mut c_void) -> c_int;
-    pub fn b200q_paged_decode_workspace_bytes(requests: usize, q_heads: usize, head_dim: usize) -> usize;
+    pub fn b200q_paged_decode_workspace_bytes(q_heads: usize, kv_heads: usize, head_dim: usize) -> usize;
     pub fn b200q_paged_decode(q: *const c_void, q_dtype: c_int, q_row_stride: i64, q_head_stride: i64, requests: usize, q_heads: usize,
                               cache: *const b200q_paged_cache, block_table: *const i32, table_row: i64, width: usize, seq_lens: *const i32,
                               scale: f32, window: usize, sinks: usize, out: *mut c_void, out_dtype: c_int, lse: *mut f32, ws: *mut c_void,
