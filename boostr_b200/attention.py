@@ -25,7 +25,8 @@ import torch
 
 from . import _cabi
 from .format import QuantError
-from .ops import _DT, _out_buffer, _require_cuda, _stream
+from .ops import _DT, _out_buffer, _require_cuda, _served, _stream
+from .tensor import hostops
 
 
 class Slots(NamedTuple):
@@ -133,6 +134,9 @@ def paged_slots(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     entered into ``block_table`` in place, -1 where the stack is empty.  ``tokens`` is the host's number of new tokens, or
     a larger one that a graph was captured with: the rows behind the last token get position 0 and slot -1.
     ``left[:1]`` is the next step's ``free_count``; ``left[1]`` is the number of pages that were missing."""
+    r = hostops().paged_slots(ctx_lens, new_lens, block_table, page_size, free_pages, free_count, tokens)
+    if _served(r):
+        return Slots(block_table, *r)
     op = "paged_slots"
     if ctx_lens.dim() != 1:
         raise QuantError(f"{op}: ctx_lens must be 1D, got {list(ctx_lens.shape)}")
@@ -166,6 +170,11 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     With ``q_weight`` / ``k_weight`` [head_dim] f32 each head is normalised first (RMSNorm).  The first 2 * cos.shape[1] elements
     are rotated by the angles of ``positions`` (``rope_tables``): elements i and i + rot / 2 together, or 2i and 2i + 1
     where ``interleaved``.  A negative slot: the token is not kept.  ``out_dtype``: q's type unless given."""
+    code = -1 if out_dtype is None else _DT.get(out_dtype)
+    if code is not None:
+        r = hostops().rope_append(q, k, v, positions, cos, sin, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, code, out)
+        if _served(r):
+            return r
     op = "rope_append"
     cache = _cache(op, k_cache, v_cache)
     d, hk = k_cache.shape[3], k_cache.shape[2]
@@ -252,6 +261,11 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     among them.  ``scale`` is head_dim ** -0.5 unless given.  ``window`` > 0: the newest ``window`` tokens and the first ``sinks`` are
     visible.  A request of length 0 (a padded row) gives zeros.  Returns out [requests, q_heads, head_dim], of q's type
     unless ``out_dtype`` says otherwise, and with ``return_lse`` also the log-sum-exp of the scores [requests, q_heads] f32."""
+    code = -1 if out_dtype is None else _DT.get(out_dtype)
+    if code is not None:
+        r = hostops().paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, code, out, return_lse)
+        if _served(r):
+            return r
     op = "paged_decode"
     cache, q, seq_lens, out, scale = _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, out, out_dtype)
     n, hq, d = q.shape
@@ -275,6 +289,11 @@ def paged_prompt(q: torch.Tensor, cu_seqlens: torch.Tensor, k_cache: torch.Tenso
     q [tokens, q_heads, head_dim] of the cache's type: rows cu_seqlens[b] .. cu_seqlens[b + 1] are the newest of the ``seq_lens[b]``
     tokens of request b, which are all in the cache.  Scale, window, sinks and results as in ``paged_decode``.  Rows of a
     request of fewer tokens than rows, and rows behind the last request, are zero."""
+    code = -1 if out_dtype is None else _DT.get(out_dtype)
+    if code is not None:
+        r = hostops().paged_prompt(q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, code, out, return_lse, cu_seqlens)
+        if _served(r):
+            return r
     op = "paged_prompt"
     cache, q, seq_lens, out, scale = _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, out, out_dtype)
     if q.dtype != k_cache.dtype:

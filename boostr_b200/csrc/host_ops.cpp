@@ -20,6 +20,7 @@
 #include <torch/version.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -388,7 +389,270 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     });
 }
 
+// ------------------------------------------------------------------------------------------ attention from a paged cache
+
+// A CUDA tensor of type t on device d; nullptr: not one.
+const at::Tensor* tensor_of(PyObject* o, at::ScalarType t, c10::Device d) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor& x = THPVariable_Unpack(o);
+    return x.defined() && x.is_cuda() && x.layout() == at::kStrided && x.device() == d && x.scalar_type() == t ? &x : nullptr;
+}
+const at::Tensor* vector_of(PyObject* o, at::ScalarType t, c10::Device d, int64_t n) {  // contiguous [n]
+    const at::Tensor* x = tensor_of(o, t, d);
+    return x && x->dim() == 1 && x->size(0) == n && x->is_contiguous() ? x : nullptr;
+}
+// Heads [rows, heads, dim] whose elements are neighbours.
+const at::Tensor* heads_of(PyObject* o) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor& x = THPVariable_Unpack(o);
+    if (!x.defined() || !x.is_cuda() || x.layout() != at::kStrided || x.dim() != 3 || x.numel() == 0 || x.stride(2) != 1) return nullptr;
+    const int c = dtype_code(x.scalar_type());
+    return c == B200Q_F32 || c == B200Q_BF16 || c == B200Q_F16 ? &x : nullptr;
+}
+bool table_of(PyObject* o, c10::Device d, int64_t requests, const at::Tensor*& t) {
+    t = tensor_of(o, at::kInt, d);
+    return t && t->dim() == 2 && t->size(0) == requests && t->size(1) > 0 && t->stride(1) == 1;
+}
+bool cache_of(PyObject* ko, PyObject* vo, c10::Device d, b200q_paged_cache& c) {
+    if (!THPVariable_CheckExact(ko) || !THPVariable_CheckExact(vo)) return false;
+    const at::Tensor &k = THPVariable_Unpack(ko), &v = THPVariable_Unpack(vo);
+    if (!k.defined() || !v.defined() || !k.is_cuda() || !v.is_cuda() || k.device() != d || v.device() != d || k.dim() != 4 || k.sizes() != v.sizes() ||
+        k.scalar_type() != v.scalar_type() || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kHalf) || k.numel() == 0 || k.stride(3) != 1 ||
+        v.stride(3) != 1)
+        return false;
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.dtype = dtype_code(k.scalar_type());
+    c.pages = (size_t)k.size(0), c.page_size = (size_t)k.size(1), c.kv_heads = (size_t)k.size(2), c.head_dim = (size_t)k.size(3);
+    for (int i = 0; i < 3; ++i) c.k_strides[i] = k.stride(i), c.v_strides[i] = v.stride(i);
+    return true;
+}
+// The output of shape `like`: `given` (a contiguous tensor of type t), or a new one of type t; false: `given` does not fit.
+bool heads_out(PyObject* given, const at::Tensor& like, at::ScalarType t, at::Tensor& out) {
+    if (given == Py_None) {
+        out = empty(like.sizes(), t, like.device());
+        return true;
+    }
+    if (!THPVariable_CheckExact(given)) return false;
+    out = THPVariable_Unpack(given);
+    return out.is_cuda() && out.device() == like.device() && out.scalar_type() == t && out.is_contiguous() && out.sizes() == like.sizes();
+}
+// A whole number that is not negative; false: not one.
+bool size_of(PyObject* o, size_t& n) {
+    const Py_ssize_t v = PyLong_CheckExact(o) ? PyLong_AsSsize_t(o) : -1;
+    if (PyErr_Occurred()) PyErr_Clear();
+    n = (size_t)v;
+    return v >= 0;
+}
+// The type that `given` / the code (-1: none) ask for, or the queries' own.
+at::ScalarType out_type(PyObject* given, long code, const at::Tensor& q) {
+    if (code >= 0) return scalar_type(code);
+    return given != Py_None && THPVariable_CheckExact(given) ? THPVariable_Unpack(given).scalar_type() : q.scalar_type();
+}
+
+// Scratch of paged_decode, apart from the other operators' because its counters are zero between calls; like theirs, one for
+// each (device, stream), and one of its own for a call that is being captured, zeroed by the graph.
+auto& g_counters = *new std::map<std::pair<int, cudaStream_t>, std::unique_ptr<Scratch>>;
+template <typename F>
+int with_counters(c10::Device dev, size_t need, F&& call) {
+    const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    if (capturing(st)) {
+        const at::Tensor buf = empty({(int64_t)need}, at::kByte, dev);
+        NoGil nogil;
+        if (cudaMemsetAsync(buf.data_ptr(), 0, B200Q_PAGED_COUNTER_BYTES, st) != cudaSuccess) return B200Q_ERR_CUDA;
+        return call(buf.data_ptr(), need, st);
+    }
+    Scratch* s;
+    {
+        std::lock_guard<std::mutex> g(g_scratch_mutex);
+        auto& e = g_counters[{dev.index(), st}];
+        if (!e) e = std::make_unique<Scratch>();
+        s = e.get();
+    }
+    NoGil nogil;
+    std::lock_guard<std::mutex> g(s->m);
+    if (!s->buf.defined() || (size_t)s->buf.numel() < need) {
+        at::Tensor buf = empty({(int64_t)need}, at::kByte, dev);
+        if (cudaMemsetAsync(buf.data_ptr(), 0, B200Q_PAGED_COUNTER_BYTES, st) != cudaSuccess) return B200Q_ERR_CUDA;
+        s->buf = buf;
+    }
+    return call(s->buf.data_ptr(), (size_t)s->buf.numel(), st);
+}
+
+// paged_slots(ctx_lens, new_lens, block_table, page_size, free_pages, free_count, tokens) -> (seq_lens, cu_seqlens, positions, slots, left)
+PyObject* paged_slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 7 || !THPVariable_CheckExact(args[0])) return not_served();
+        const at::Tensor& first = THPVariable_Unpack(args[0]);
+        if (!first.defined() || !first.is_cuda() || first.dim() != 1) return not_served();
+        const c10::Device d = first.device();
+        const int64_t n = first.size(0);
+        const at::Tensor *ctx = vector_of(args[0], at::kInt, d, n), *fresh = vector_of(args[1], at::kInt, d, n), *table, *free = tensor_of(args[4], at::kInt, d),
+                         *count = vector_of(args[5], at::kInt, d, 1);
+        size_t page, tokens;
+        if (!n || !ctx || !fresh || !free || !count || free->dim() != 1 || !free->is_contiguous() || !table_of(args[2], d, n, table) ||
+            !size_of(args[3], page) || !page || !size_of(args[6], tokens))
+            return not_served();
+        DeviceScope dev(d);
+        const at::Tensor out[5] = {empty({n}, at::kInt, d), empty({n + 1}, at::kInt, d), empty({(int64_t)tokens}, at::kInt, d),
+                                   empty({(int64_t)tokens}, at::kLong, d), empty({2}, at::kInt, d)};
+        const int rc = with_scratch(d, 0, [&](void*, size_t, cudaStream_t st) {
+            return b200q_paged_slots(ctx->data_ptr<int>(), fresh->data_ptr<int>(), (size_t)n, table->data_ptr<int>(), table->stride(0), (size_t)table->size(1),
+                                     page, free->data_ptr<int>(), (size_t)free->numel(), count->data_ptr<int>(), out[0].data_ptr<int>(),
+                                     out[1].data_ptr<int>(), out[2].data_ptr<int>(), out[3].data_ptr<int64_t>(), tokens, out[4].data_ptr<int>(), st);
+        });
+        if (rc != B200Q_OK) return PyLong_FromLong(rc);
+        PyObject* r = PyTuple_New(5);
+        if (!r) return nullptr;
+        for (int i = 0; i < 5; ++i) {
+            PyObject* o = THPVariable_Wrap(out[i]);
+            if (!o) {
+                Py_DECREF(r);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(r, i, o);
+        }
+        return r;
+    });
+}
+
+// rope_append(q, k, v, positions, cos, sin, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, out dtype code or -1, out or None)
+PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 15) return not_served();
+        const at::Tensor *q = heads_of(args[0]), *k = heads_of(args[1]), *v = heads_of(args[2]);
+        b200q_paged_cache c;
+        if (!q || !k || !v || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type()) return not_served();
+        const c10::Device d = q->device();
+        const int64_t t = q->size(0);
+        if (k->device() != d || v->device() != d || !cache_of(args[6], args[7], d, c)) return not_served();
+        const int64_t hk = (int64_t)c.kv_heads, dim = (int64_t)c.head_dim;
+        for (const at::Tensor* x : {k, v})
+            if (x->size(0) != t || x->size(1) != hk || x->size(2) != dim) return not_served();
+        const at::Tensor *pos = vector_of(args[3], at::kInt, d, t), *slots = vector_of(args[8], at::kLong, d, t), *cos = tensor_of(args[4], at::kFloat, d),
+                         *sin = tensor_of(args[5], at::kFloat, d);
+        if (q->size(2) != dim || !pos || !slots || !cos || !sin || cos->dim() != 2 || cos->sizes() != sin->sizes() || !cos->is_contiguous() ||
+            !sin->is_contiguous() || 2 * cos->size(1) > dim)
+            return not_served();
+        const float* w[2] = {nullptr, nullptr};
+        for (int i = 0; i < 2; ++i)
+            if (args[9 + i] != Py_None) {
+                const at::Tensor* x = vector_of(args[9 + i], at::kFloat, d, dim);
+                if (!x) return not_served();
+                w[i] = x->data_ptr<float>();
+            }
+        const float eps = (float)PyFloat_AsDouble(args[11]);
+        const int inter = PyObject_IsTrue(args[12]);
+        const long code = PyLong_AsLong(args[13]);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            return not_served();
+        }
+        const at::ScalarType ot = out_type(args[14], code, *q);
+        const int odt = dtype_code(ot);
+        DeviceScope dev(d);
+        at::Tensor out;
+        if (odt < 0 || odt == B200Q_F64 || !heads_out(args[14], *q, ot, out)) return not_served();
+        const b200q_heads h[3] = {{q->data_ptr(), q->stride(0), q->stride(1)}, {k->data_ptr(), k->stride(0), k->stride(1)}, {v->data_ptr(), v->stride(0), v->stride(1)}};
+        const int rc = with_scratch(d, 0, [&](void*, size_t, cudaStream_t st) {
+            return b200q_rope_append(h, h + 1, h + 2, dtype_code(q->scalar_type()), (size_t)t, (size_t)q->size(1), pos->data_ptr<int>(), cos->data_ptr<float>(),
+                                     sin->data_ptr<float>(), (size_t)cos->size(0), (size_t)(2 * cos->size(1)), inter, w[0], w[1], eps, &c,
+                                     slots->data_ptr<int64_t>(), out.data_ptr(), odt, st);
+        });
+        return result(rc, out);
+    });
+}
+
+// What the two attentions share: arguments q, k_cache, v_cache, block_table, seq_lens, scale or None, window, sinks, out dtype code or -1,
+// out or None, log-sum-exp wanted, starting at args[0]
+struct Attn {
+    const at::Tensor *q, *table, *lens;
+    b200q_paged_cache c;
+    float scale;
+    size_t window, sinks;
+    int odt;
+    at::Tensor out, lse;
+};
+bool attn_of(PyObject* const* args, Attn& a) {
+    a.q = heads_of(args[0]);
+    if (!a.q || !cache_of(args[1], args[2], a.q->device(), a.c)) return false;
+    const at::Tensor& q = *a.q;
+    const c10::Device d = q.device();
+    a.lens = tensor_of(args[4], at::kInt, d);
+    if (!a.lens || a.lens->dim() != 1 || !a.lens->is_contiguous() || !table_of(args[3], d, a.lens->size(0), a.table)) return false;
+    const int qdt = dtype_code(q.scalar_type());
+    const int64_t unit = qdt == B200Q_F32 ? 4 : 8;
+    if (q.size(2) != (int64_t)a.c.head_dim || q.size(1) % (int64_t)a.c.kv_heads || (qdt != B200Q_F32 && qdt != a.c.dtype) || q.stride(0) % unit ||
+        q.stride(1) % unit || (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15))
+        return false;
+    a.scale = args[5] == Py_None ? (float)std::pow((double)a.c.head_dim, -0.5) : (float)PyFloat_AsDouble(args[5]);
+    const long code = PyLong_AsLong(args[8]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    if (!size_of(args[6], a.window) || !size_of(args[7], a.sinks)) return false;
+    const at::ScalarType ot = out_type(args[9], code, q);
+    a.odt = dtype_code(ot);
+    if (a.odt < 0 || a.odt == B200Q_F64 || !heads_out(args[9], q, ot, a.out)) return false;
+    if (PyObject_IsTrue(args[10])) a.lse = empty({q.size(0), q.size(1)}, at::kFloat, d);
+    return true;
+}
+PyObject* attn_result(int rc, const Attn& a) {
+    if (rc != B200Q_OK) return PyLong_FromLong(rc);
+    if (!a.lse.defined()) return THPVariable_Wrap(a.out);
+    PyObject *o = THPVariable_Wrap(a.out), *l = THPVariable_Wrap(a.lse);
+    PyObject* r = o && l ? PyTuple_Pack(2, o, l) : nullptr;
+    Py_XDECREF(o);
+    Py_XDECREF(l);
+    return r;
+}
+
+PyObject* paged_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        Attn a;
+        if (nargs != 11 || !THPVariable_CheckExact(args[0]) || !THPVariable_Unpack(args[0]).is_cuda()) return not_served();
+        const c10::Device d = THPVariable_Unpack(args[0]).device();
+        DeviceScope dev(d);
+        if (!attn_of(args, a) || a.lens->size(0) != a.q->size(0)) return not_served();
+        const size_t need = b200q_paged_decode_workspace_bytes((size_t)a.q->size(1), a.c.kv_heads, a.c.head_dim);
+        if (!need) return not_served();
+        const int rc = with_counters(d, need, [&](void* ws, size_t bytes, cudaStream_t st) {
+            return b200q_paged_decode(a.q->data_ptr(), dtype_code(a.q->scalar_type()), a.q->stride(0), a.q->stride(1), (size_t)a.q->size(0),
+                                      (size_t)a.q->size(1), &a.c, a.table->data_ptr<int>(), a.table->stride(0), (size_t)a.table->size(1),
+                                      a.lens->data_ptr<int>(), a.scale, a.window, a.sinks, a.out.data_ptr(), a.odt,
+                                      a.lse.defined() ? a.lse.data_ptr<float>() : nullptr, ws, bytes, st);
+        });
+        return attn_result(rc, a);
+    });
+}
+
+// paged_prompt(q, k_cache, ..., as above, cu_seqlens)
+PyObject* paged_prompt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        Attn a;
+        if (nargs != 12 || !THPVariable_CheckExact(args[0]) || !THPVariable_Unpack(args[0]).is_cuda()) return not_served();
+        const c10::Device d = THPVariable_Unpack(args[0]).device();
+        DeviceScope dev(d);
+        if (!attn_of(args, a) || a.q->scalar_type() == at::kFloat) return not_served();
+        const at::Tensor* cu = vector_of(args[11], at::kInt, d, a.lens->size(0) + 1);
+        if (!cu) return not_served();
+        const int rc = with_scratch(d, 0, [&](void*, size_t, cudaStream_t st) {
+            return b200q_paged_prompt(a.q->data_ptr(), dtype_code(a.q->scalar_type()), a.q->stride(0), a.q->stride(1), (size_t)a.q->size(0),
+                                      (size_t)a.q->size(1), cu->data_ptr<int>(), (size_t)a.lens->size(0), &a.c, a.table->data_ptr<int>(), a.table->stride(0),
+                                      (size_t)a.table->size(1), a.lens->data_ptr<int>(), a.scale, a.window, a.sinks, a.out.data_ptr(), a.odt,
+                                      a.lse.defined() ? a.lse.data_ptr<float>() : nullptr, st);
+        });
+        return attn_result(rc, a);
+    });
+}
+
+#define FASTCALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
+    FASTCALL(paged_slots),
+    FASTCALL(rope_append),
+    FASTCALL(paged_decode),
+    FASTCALL(paged_prompt),
     {"make_ref", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(make_ref)), METH_FASTCALL, nullptr},
     {"quant_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quant_matmul)), METH_FASTCALL, nullptr},
     {"quant_matmul_batch", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quant_matmul_batch)), METH_FASTCALL, nullptr},
@@ -396,6 +660,7 @@ PyMethodDef methods[] = {
     {"quant_mlp", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quant_mlp)), METH_FASTCALL, nullptr},
     {"dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(dequantize)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
+#undef FASTCALL
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostops", nullptr, -1, methods};
 
 }  // namespace

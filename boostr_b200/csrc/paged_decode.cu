@@ -36,7 +36,7 @@ constexpr float WEIGHT_BIAS = F16 ? 14.f : 0.f;
 
 struct TileMeta {
     int valid;            // keys of the warp's 16 that are visible
-    uint32_t b, item;
+    uint32_t b, h, h0;    // request, key-value head, first of the query heads that share it
     uint32_t t, nt;       // tile of its item, and their number
 };
 
@@ -157,42 +157,46 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
     const uint32_t ntiles = (uint32_t)(end - begin);
 
     // ---- the cursor of the copies: the next tile whose page numbers are fetched
-    uint32_t c_b = s_first[0], c_item, c_t, c_nt, c_sinks, c_from, c_n, c_left = ntiles;
+    uint32_t c_b = s_first[0], c_h, c_h0, c_t, c_nt, c_sinks, c_from, c_n, c_left = ntiles;
     visible_keys(p, attn_len(p, c_b), c_sinks, c_from, c_n);
     c_nt = (c_n + DEC_TILE - 1) / DEC_TILE;
-    c_item = s_first[1] / c_nt;
-    c_t = s_first[1] - c_item * c_nt;
-    // lanes 0 to 15: where the keys of the warp's 16 lie, lanes 16 to 31: the values (-1: not visible)
-    int64_t off = -1;
+    c_t = s_first[1] % c_nt;
+    c_h = s_first[1] / c_nt / d.chunks;
+    c_h0 = (s_first[1] / c_nt - c_h * d.chunks) * HEADS;
+    // page and place in it of key lane % 16 of the warp's 16 in the next tile (page < 0: not visible).  Read one tile ahead and
+    // not looked at before its copies are issued, so that no step waits for the table.
+    int32_t page = -1;
+    uint32_t tok = 0;
     TileMeta next;
     auto fetch = [&]() {
-        off = -1;
+        page = -1;
         if (c_left == 0) return;
         --c_left;
         const uint32_t v0 = c_t * DEC_TILE + warp * 16, i = v0 + (lane & 15);
         if (i < c_n) {
-            const uint32_t j = i < c_sinks ? i : i - c_sinks + c_from;
-            uint32_t page, tok;
-            if (attn_page(p, c_b, j, page, tok)) {
-                const uint32_t h = c_item / d.chunks;
-                off = lane < 16 ? (int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)h * p.k_head
-                                : (int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)h * p.v_head;
-            }
+            const uint32_t j = i < c_sinks ? i : i - c_sinks + c_from, e = p.page.div(j);
+            tok = j - e * p.page.d;
+            page = p.table[(int64_t)c_b * p.table_row + e];
         }
         next.valid = min(16, max(0, (int)c_n - (int)v0));
         next.b = c_b;
-        next.item = c_item;
+        next.h = c_h;
+        next.h0 = c_h0;
         next.t = c_t;
         next.nt = c_nt;
         if (++c_t == c_nt) {
             c_t = 0;
-            if (++c_item == d.items && c_left) {
-                c_item = 0;
-                do {
-                    ++c_b;
-                    visible_keys(p, attn_len(p, c_b), c_sinks, c_from, c_n);
-                } while (c_n == 0);
-                c_nt = (c_n + DEC_TILE - 1) / DEC_TILE;
+            c_h0 += HEADS;
+            if (c_h0 >= p.group) {
+                c_h0 = 0;
+                if (++c_h == p.hkv && c_left) {
+                    c_h = 0;
+                    do {
+                        ++c_b;
+                        visible_keys(p, attn_len(p, c_b), c_sinks, c_from, c_n);
+                    } while (c_n == 0);
+                    c_nt = (c_n + DEC_TILE - 1) / DEC_TILE;
+                }
             }
         }
     };
@@ -206,6 +210,12 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
             --to_issue;
             if (lane == 0) meta[s] = next;
             const uint32_t dst = ring + s * Sh::STAGE;
+            // lanes 0 to 15: where the keys lie, lanes 16 to 31: the values
+            int64_t off = -1;
+            if ((uint32_t)page < p.pages)
+                off = lane < 16 ? (int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)next.h * p.k_head
+                                : (int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)next.h * p.v_head;
+            else if ((lane & 15) < next.valid) atomicOr(p.status, STATUS_BAD_INDEX);
 #pragma unroll
             for (int r = 0; r < 16; r += ROWS_PER) {
                 const uint32_t row = r + my_row;
@@ -230,8 +240,7 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
         cp_async_wait<STAGES - 1>();
         __syncwarp();
         const TileMeta mt = meta[s];
-        const uint32_t b = mt.b, h = mt.item / d.chunks, h0 = (mt.item - h * d.chunks) * HEADS;  // first query head of the group
-        const uint32_t heads = min((uint32_t)HEADS, p.group - h0);
+        const uint32_t b = mt.b, h = mt.h, h0 = mt.h0, heads = min((uint32_t)HEADS, p.group - h0);
         if (fresh) {
             fresh = false;
             begins = mt.t == 0;
@@ -275,9 +284,13 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
         const uint32_t kt = ring + s * Sh::STAGE, vt = kt + 16 * ROW;
         if (mt.valid > 0) {
             // ---- scores: 16 keys x heads
-            float sc[NT][4];
+            // partial sums of each term, and of even and odd k steps: products that wait for one another cost more than the adds
+            constexpr int CH = NT == 1 && DP <= 128 ? 2 : 1;
+            float part[CH * TERMS][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+            for (int c = 0; c < CH * TERMS; ++c)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) part[c][nt][0] = part[c][nt][1] = part[c][nt][2] = part[c][nt][3] = 0.f;
             {
                 const uint32_t row = (lane & 7) + (lane & 8);
 #pragma unroll
@@ -289,13 +302,22 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             const uint2 q = qf[((ks * TERMS + t) * NT + nt) * 32 + lane];
-                            mma16<F16>(sc[nt], a, q.x, q.y);
+                            mma16<F16>(part[CH * t + (ks & (CH - 1))][nt], a, q.x, q.y);
                         }
                 }
             }
+            float sc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    sc[nt][c] = 0.f;
+#pragma unroll
+                    for (int t = CH * TERMS - 1; t >= 0; --t) sc[nt][c] += part[t][nt][c];  // the smallest terms first
+                }
             // ---- softmax: element c of a lane is key lane / 4 + 8 (c / 2), head 2 (lane % 4) + c % 2 of its eight
             const bool in0 = (lane >> 2) < mt.valid, in1 = (lane >> 2) + 8 < mt.valid;
-            uint32_t ph[NT][2], pl[NT][2];
+            uint32_t pt[TERMS][NT][2];  // the weights as a sum of 16-bit terms, too
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float x[4], alpha[2];
@@ -317,11 +339,14 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t r = pack2<F16>(x[2 * j], x[2 * j + 1]);
-                    ph[nt][j] = transpose8(r);
-                    if constexpr (SPLIT) {
-                        const float2 a = unpack2<F16>(r);
-                        pl[nt][j] = transpose8(pack2<F16>(x[2 * j] - a.x, x[2 * j + 1] - a.y));
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const uint32_t r = pack2<F16>(x[2 * j], x[2 * j + 1]);
+                        pt[t][nt][j] = transpose8(r);
+                        if constexpr (TERMS > 1) {
+                            const float2 a = unpack2<F16>(r);
+                            x[2 * j] -= a.x, x[2 * j + 1] -= a.y;
+                        }
                     }
                 }
                 if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.f || alpha[1] != 1.f)) {
@@ -341,10 +366,9 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                 uint32_t a[4];
                 ldsm_x4_t(a, vt + key * ROW + (((2 * k + ((lane >> 3) & 1)) ^ (key & 7)) << 4));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma16<F16>(o[k][nt], a, ph[nt][0], ph[nt][1]);
-                    if constexpr (SPLIT) mma16<F16>(o[k][nt], a, pl[nt][0], pl[nt][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) mma16<F16>(o[k][nt], a, pt[t][nt][0], pt[t][nt][1]);
             }
         }
         if (mt.t + 1 == mt.nt || i + 1 == ntiles) {

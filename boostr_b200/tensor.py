@@ -25,6 +25,7 @@ class _PythonForms:
         return NotImplemented
 
     make_ref = quant_matmul = quant_matmul_batch = quant_swiglu = quant_mlp = dequantize = _decline
+    paged_slots = rope_append = paged_decode = paged_prompt = _decline
 
 
 def hostops():
