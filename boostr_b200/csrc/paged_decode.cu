@@ -317,25 +317,24 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                 }
             // ---- softmax: element c of a lane is key lane / 4 + 8 (c / 2), head 2 (lane % 4) + c % 2 of its eight
             const bool in0 = (lane >> 2) < mt.valid, in1 = (lane >> 2) + 8 < mt.valid;
+            float alpha[NT][2];
             uint32_t pt[TERMS][NT][2];  // the weights as a sum of 16-bit terms, too
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float x[4], alpha[2];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] = (c < 2 ? in0 : in1) ? sc[nt][c] * p.scale_log2 : -INFINITY;
+                float x[4];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float mx = fmaxf(x[c], x[c + 2]);
+                    float mx = fmaxf(in0 ? sc[nt][c] * p.scale_log2 : -INFINITY, in1 ? sc[nt][c + 2] * p.scale_log2 : -INFINITY);
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
                     mx = fmaxf(mx, m[nt][c]);
-                    alpha[c] = mx == -INFINITY ? 1.f : exp2_approx(m[nt][c] - mx);
+                    alpha[nt][c] = mx == -INFINITY ? 1.f : exp2_approx(m[nt][c] - mx);
                     m[nt][c] = mx;
                     const float base = mx == -INFINITY ? 0.f : mx - WEIGHT_BIAS<F16>;
-                    x[c] = exp2_approx(x[c] - base);
-                    x[c + 2] = exp2_approx(x[c + 2] - base);
-                    l[nt][c] = fmaf(l[nt][c], alpha[c], x[c] + x[c + 2]);
+                    x[c] = in0 ? exp2_approx(fmaf(sc[nt][c], p.scale_log2, -base)) : 0.f;
+                    x[c + 2] = in1 ? exp2_approx(fmaf(sc[nt][c + 2], p.scale_log2, -base)) : 0.f;
+                    l[nt][c] = fmaf(l[nt][c], alpha[nt][c], x[c] + x[c + 2]);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -349,13 +348,12 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                         }
                     }
                 }
-                if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+                if constexpr (!SPLIT) {
+                    if (__any_sync(0xFFFFFFFFu, alpha[nt][0] != 1.f || alpha[nt][1] != 1.f)) {
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        o[k][nt][0] *= alpha[0];
-                        o[k][nt][1] *= alpha[1];
-                        o[k][nt][2] *= alpha[0];
-                        o[k][nt][3] *= alpha[1];
+                        for (int k = 0; k < KS; ++k)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) o[k][nt][c] *= alpha[nt][c & 1];
                     }
                 }
             }
@@ -366,9 +364,19 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                 uint32_t a[4];
                 ldsm_x4_t(a, vt + key * ROW + (((2 * k + ((lane >> 3) & 1)) ^ (key & 7)) << 4));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt) {
+                    if constexpr (!SPLIT) {
+                        mma16<F16>(o[k][nt], a, pt[0][nt][0], pt[0][nt][1]);
+                    } else {
+                        // the tensor core cuts its sums off: over a long row that would show in an f32 result, so a tile is summed by
+                        // itself, smallest terms first, and added with rounding
+                        float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int t = 0; t < TERMS; ++t) mma16<F16>(o[k][nt], a, pt[t][nt][0], pt[t][nt][1]);
+                        for (int t = TERMS - 1; t >= 0; --t) mma16<F16>(x, a, pt[t][nt][0], pt[t][nt][1]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[k][nt][c] = fmaf(o[k][nt][c], alpha[nt][c & 1], x[c]);
+                    }
+                }
             }
         }
         if (mt.t + 1 == mt.nt || i + 1 == ntiles) {
