@@ -3,12 +3,12 @@
 //
 // Bound: HBM reads of the keys and values (two bytes an element for 2 group flops each; the group's query heads share every
 // byte).  The keys that a request sees (its sinks, then its window) are numbered through without a gap, cut into tiles of
-// 64, and all tiles of the batch, request by request and head by head, are laid end to end; every CTA takes an equal run of
+// 64 (128 of narrow heads), and all tiles of the batch, request by request and head by head, are laid end to end; every CTA takes an equal run of
 // them, so ragged batches and single long requests are balanced alike and the lengths are needed on the GPU only.
 // Where a run ends inside a head, the CTAs that share the head leave partial sums in scratch, and the one that finishes last
 // adds them up in their order (the result does not depend on which one that is).
 //
-// In a tile each of four warps owns 16 keys, with a ring of its own filled by asynchronous 16-byte copies (zeros where a key
+// In a tile each of four warps owns 16 keys (32 of narrow heads), with a ring of its own filled by asynchronous 16-byte copies (zeros where a key
 // is not visible, so nothing that lies in unused places of a page can reach a sum); no barrier separates the warps until
 // their sums are joined at the end of a head.  Products on mma.sync with the keys as the 16 rows and 8 query heads as the
 // columns: S^T = K Q^T, O^T = V^T P^T; at two flops a byte and head the tensor cores idle at any rate, and the operands come
@@ -28,11 +28,14 @@ struct DecodePlan {
 namespace {
 
 constexpr size_t DEC_COUNTER_BYTES = 4096;  // one counter for each CTA, zero between calls
-constexpr int DEC_WARPS = 4, DEC_THREADS = 32 * DEC_WARPS, DEC_TILE = 16 * DEC_WARPS;
+constexpr int DEC_WARPS = 4, DEC_THREADS = 32 * DEC_WARPS;
 
-// f16 weights are kept 2^14 times their size: their subnormals would otherwise lose the small ones of a long row
+// The maximum that weights are taken against follows a row's scores only when one exceeds it by 2^SLACK: a vote in place of a
+// reduction across lanes and a rescaling of the sums in almost every tile, for weights of up to 2^SLACK.
+constexpr float SLACK = 5.f;
+// f16 weights are kept 2^9 times their size (2^14 with the slack): their subnormals would otherwise lose the small ones of a long row
 template <bool F16>
-constexpr float WEIGHT_BIAS = F16 ? 14.f : 0.f;
+constexpr float WEIGHT_BIAS = F16 ? 9.f : 0.f;
 
 struct TileMeta {
     int valid;            // keys of the warp's 16 that are visible
@@ -43,8 +46,11 @@ struct TileMeta {
 template <int DP, int NT, bool F16, bool SPLIT>
 struct DecodeShape {
     static constexpr int KS = DP / 16, TERMS = SPLIT ? (F16 ? 2 : 3) : 1, HEADS = 8 * NT;
-    static constexpr int ROW = DP * 2, WARP_STAGE = 2 * 16 * ROW, STAGE = DEC_WARPS * WARP_STAGE;
-    static constexpr int STAGES = DP == 64 ? 4 : 3;
+    static constexpr int KPW = DP == 64 ? 32 : 16, TILE = KPW * DEC_WARPS;  // keys of a warp, and of a CTA, in a tile
+    static constexpr int CTAS = DP <= 128 ? 2 : 1;                          // of an SM
+    static constexpr int ROW = DP * 2, WARP_STAGE = 2 * KPW * ROW, STAGE = DEC_WARPS * WARP_STAGE;
+    static constexpr int STAGES = 3;
+    static constexpr bool Q_REGS = KS * TERMS * NT <= 8;  // the query operand fits into registers beside the sums
     static constexpr int Q_BYTES = KS * TERMS * NT * 32 * 8;
     static constexpr int OFF_Q = STAGES * STAGE, OFF_ML = OFF_Q + Q_BYTES, OFF_META = OFF_ML + DEC_WARPS * HEADS * 8,
                          SMEM = OFF_META + DEC_WARPS * STAGES * (int)sizeof(TileMeta);
@@ -77,11 +83,51 @@ __device__ __forceinline__ void write_row(const AttnParams& p, uint32_t b, uint3
     }
 }
 
-template <int DP, int NT, bool F16, bool SPLIT, int MINB>
-__global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnParams p, const DecodePlan d) {
+// 64-bit value of another lane
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, uint32_t lane) {
+    const uint32_t lo = __shfl_sync(0xFFFFFFFFu, (uint32_t)v, lane), hi = __shfl_sync(0xFFFFFFFFu, (uint32_t)(v >> 32), lane);
+    return ((uint64_t)hi << 32) | lo;
+}
+
+// Adds up the parts of CTAs first .. last of elements dim .. dim + 3 of a head, in that order.
+template <int HEADS, int DP>
+__device__ __forceinline__ void join_parts(const float* parts, uint32_t first, uint32_t last, uint32_t head, uint32_t dim, float4& a, float& mx, float& sum) {
+    constexpr int AT_ONCE = 16, PART = HEADS * (DP + 2);
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
+    mx = -INFINITY, sum = 0.f;
+    for (uint32_t c0 = first; c0 <= last; c0 += AT_ONCE) {
+        float4 x[AT_ONCE];
+        float pm[AT_ONCE], ps[AT_ONCE], top = mx;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            pm[u] = -INFINITY, ps[u] = 0.f, x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c0 + u <= last) {
+                const float* q = parts + (size_t)(2 * (c0 + u) + (c0 + u == first ? 1 : 0)) * PART;
+                x[u] = __ldcg(reinterpret_cast<const float4*>(q + head * DP + dim));
+                pm[u] = __ldcg(q + HEADS * DP + head);
+                ps[u] = __ldcg(q + HEADS * DP + HEADS + head);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) top = fmaxf(top, pm[u]);
+        const float f0 = mx == -INFINITY ? 0.f : exp2_approx(mx - top);
+        a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0, sum *= f0;
+        mx = top;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const float f = pm[u] == -INFINITY ? 0.f : exp2_approx(pm[u] - top);
+            a.x = fmaf(x[u].x, f, a.x), a.y = fmaf(x[u].y, f, a.y), a.z = fmaf(x[u].z, f, a.z), a.w = fmaf(x[u].w, f, a.w);
+            sum = fmaf(ps[u], f, sum);
+        }
+    }
+}
+
+template <int DP, int NT, bool F16, bool SPLIT>
+__global__ void __launch_bounds__(DEC_THREADS, DecodeShape<DP, NT, F16, SPLIT>::CTAS) decode_kernel(const AttnParams p, const DecodePlan d) {
     using Sh = DecodeShape<DP, NT, F16, SPLIT>;
-    constexpr int KS = Sh::KS, TERMS = Sh::TERMS, STAGES = Sh::STAGES, ROW = Sh::ROW, HEADS = Sh::HEADS;
-    constexpr int CPR = ROW / 16, ROWS_PER = 32 / CPR > 0 ? 32 / CPR : 1;  // 16-byte chunks of a row; rows of one copy instruction
+    constexpr int KS = Sh::KS, TERMS = Sh::TERMS, STAGES = Sh::STAGES, ROW = Sh::ROW, HEADS = Sh::HEADS, KPW = Sh::KPW, MT = KPW / 16, TILE = Sh::TILE;
+    constexpr int CPR = ROW / 16, ROWS_PER = 32 / CPR;  // 16-byte chunks of a row; rows of one copy instruction
+    constexpr int QN = KS * NT * 32 / DEC_THREADS;      // entries of the query operand for each thread
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t sbase = smem_u32(smem);
@@ -89,7 +135,7 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
     float2* ml = reinterpret_cast<float2*>(smem + Sh::OFF_ML);
     TileMeta* meta = reinterpret_cast<TileMeta*>(smem + Sh::OFF_META) + warp * STAGES;
     __shared__ uint64_t s_scan[DEC_WARPS];
-    __shared__ uint32_t s_first[2];
+    __shared__ uint32_t s_first[3];
     __shared__ uint32_t s_last;
 
     grid_dep_wait();
@@ -102,10 +148,14 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
         const uint32_t chunk = (p.requests + DEC_THREADS - 1) / DEC_THREADS;
         const uint32_t b0 = min(p.requests, threadIdx.x * chunk), b1 = min(p.requests, b0 + chunk);
         uint64_t sum = 0;
+        uint32_t n = 0;
+        bool empty = false;
         for (uint32_t b = b0; b < b1; ++b) {
-            uint32_t sk, fr, n;
-            visible_keys(p, attn_len(p, b), sk, fr, n);
-            sum += (n + DEC_TILE - 1) / DEC_TILE;
+            uint32_t sk, fr;
+            const uint32_t len = attn_len(p, b);
+            visible_keys(p, len, sk, fr, n);
+            sum += (n + TILE - 1) / TILE;
+            empty |= n == 0;
         }
         uint64_t s = sum;
 #pragma unroll
@@ -114,7 +164,7 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
             if (lane >= i) s += o;
         }
         if (lane == 31) s_scan[warp] = s;
-        __syncthreads();
+        const bool empties = __syncthreads_or(empty);
         uint64_t before = 0;
         total = 0;
 #pragma unroll
@@ -123,8 +173,7 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
             total += s_scan[w];
         }
         total *= d.items;
-        const uint64_t runs = (total + d.min_tiles - 1) / d.min_tiles;
-        active = (uint32_t)min((uint64_t)gridDim.x, runs);
+        active = (uint32_t)min((uint64_t)gridDim.x, (total + d.min_tiles - 1) / d.min_tiles);
         begin = end = 0;
         if (blockIdx.x < active) {
             begin = blockIdx.x * total / active;
@@ -133,9 +182,9 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
         uint64_t pre = (before + s - sum) * d.items;  // tiles before request b0
         if (begin < end && begin >= pre && begin < pre + sum * d.items) {
             for (uint32_t b = b0; b < b1; ++b) {
-                uint32_t sk, fr, n;
-                visible_keys(p, attn_len(p, b), sk, fr, n);
-                const uint64_t t = (uint64_t)((n + DEC_TILE - 1) / DEC_TILE) * d.items;
+                uint32_t sk, fr;
+                if (chunk > 1) visible_keys(p, attn_len(p, b), sk, fr, n);
+                const uint64_t t = (uint64_t)((n + TILE - 1) / TILE) * d.items;
                 if (begin < pre + t) {
                     s_first[0] = b;
                     s_first[1] = (uint32_t)(begin - pre);
@@ -144,26 +193,26 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                 pre += t;
             }
         }
+        if (empties)  // requests that see nothing
+            for (uint32_t b = blockIdx.x; b < p.requests; b += gridDim.x)
+                if (p.lens[b] <= 0) {
+                    for (uint32_t i = threadIdx.x; i < p.hq * p.dim; i += DEC_THREADS) store_f32(p.out, (int64_t)b * p.hq * p.dim + i, p.out_dtype, 0.f);
+                    if (p.lse)
+                        for (uint32_t i = threadIdx.x; i < p.hq; i += DEC_THREADS) p.lse[(int64_t)b * p.hq + i] = -INFINITY;
+                }
         __syncthreads();
     }
-    // requests that see nothing
-    for (uint32_t b = blockIdx.x; b < p.requests; b += gridDim.x)
-        if (p.lens[b] <= 0) {
-            for (uint32_t i = threadIdx.x; i < p.hq * p.dim; i += DEC_THREADS) store_f32(p.out, (int64_t)b * p.hq * p.dim + i, p.out_dtype, 0.f);
-            if (p.lse)
-                for (uint32_t i = threadIdx.x; i < p.hq; i += DEC_THREADS) p.lse[(int64_t)b * p.hq + i] = -INFINITY;
-        }
     if (begin >= end) return;
     const uint32_t ntiles = (uint32_t)(end - begin);
 
     // ---- the cursor of the copies: the next tile whose page numbers are fetched
     uint32_t c_b = s_first[0], c_h, c_h0, c_t, c_nt, c_sinks, c_from, c_n, c_left = ntiles;
     visible_keys(p, attn_len(p, c_b), c_sinks, c_from, c_n);
-    c_nt = (c_n + DEC_TILE - 1) / DEC_TILE;
+    c_nt = (c_n + TILE - 1) / TILE;
     c_t = s_first[1] % c_nt;
     c_h = s_first[1] / c_nt / d.chunks;
     c_h0 = (s_first[1] / c_nt - c_h * d.chunks) * HEADS;
-    // page and place in it of key lane % 16 of the warp's 16 in the next tile (page < 0: not visible).  Read one tile ahead and
+    // page and place in it of key lane % KPW of the warp's in the next tile (page < 0: not visible).  Read one tile ahead and
     // not looked at before its copies are issued, so that no step waits for the table.
     int32_t page = -1;
     uint32_t tok = 0;
@@ -172,13 +221,13 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
         page = -1;
         if (c_left == 0) return;
         --c_left;
-        const uint32_t v0 = c_t * DEC_TILE + warp * 16, i = v0 + (lane & 15);
+        const uint32_t v0 = c_t * TILE + warp * KPW, i = v0 + (lane & (KPW - 1));
         if (i < c_n) {
             const uint32_t j = i < c_sinks ? i : i - c_sinks + c_from, e = p.page.div(j);
             tok = j - e * p.page.d;
             page = p.table[(int64_t)c_b * p.table_row + e];
         }
-        next.valid = min(16, max(0, (int)c_n - (int)v0));
+        next.valid = min(KPW, max(0, (int)c_n - (int)v0));
         next.b = c_b;
         next.h = c_h;
         next.h0 = c_h0;
@@ -195,7 +244,7 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                         ++c_b;
                         visible_keys(p, attn_len(p, c_b), c_sinks, c_from, c_n);
                     } while (c_n == 0);
-                    c_nt = (c_n + DEC_TILE - 1) / DEC_TILE;
+                    c_nt = (c_n + TILE - 1) / TILE;
                 }
             }
         }
@@ -210,29 +259,71 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
             --to_issue;
             if (lane == 0) meta[s] = next;
             const uint32_t dst = ring + s * Sh::STAGE;
-            // lanes 0 to 15: where the keys lie, lanes 16 to 31: the values
-            int64_t off = -1;
-            if ((uint32_t)page < p.pages)
-                off = lane < 16 ? (int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)next.h * p.k_head
-                                : (int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)next.h * p.v_head;
-            else if ((lane & 15) < next.valid) atomicOr(p.status, STATUS_BAD_INDEX);
+            // where the lane's key and value lie; 0: not visible
+            uint64_t ka = 0, va = 0;
+            if ((uint32_t)page < p.pages) {
+                ka = reinterpret_cast<uint64_t>(p.k) + 2 * ((int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)next.h * p.k_head);
+                va = reinterpret_cast<uint64_t>(p.v) + 2 * ((int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)next.h * p.v_head);
+            } else if ((lane & (KPW - 1)) < next.valid) {
+                atomicOr(p.status, STATUS_BAD_INDEX);
+            }
 #pragma unroll
-            for (int r = 0; r < 16; r += ROWS_PER) {
+            for (int r = 0; r < KPW; r += ROWS_PER) {
                 const uint32_t row = r + my_row;
-                const uint32_t at = row * ROW + ((my_chunk ^ (row & 7)) << 4);
-                const int64_t ko = __shfl_sync(0xFFFFFFFFu, off, row), vo = __shfl_sync(0xFFFFFFFFu, off, 16 + row);
-                cp_async16(dst + at, p.k + (ko >= 0 && in_dim ? (ko + my_chunk * 8) * 2 : 0), ko >= 0 && in_dim ? 16 : 0);
-                cp_async16(dst + 16 * ROW + at, p.v + (vo >= 0 && in_dim ? (vo + my_chunk * 8) * 2 : 0), vo >= 0 && in_dim ? 16 : 0);
+                const uint32_t at = dst + row * ROW + ((my_chunk ^ (row & 7)) << 4);
+                const uint64_t k1 = shfl64(ka, row);
+                const uint32_t bytes = k1 && in_dim ? 16 : 0;
+                cp_async16(at, reinterpret_cast<const void*>(bytes ? k1 + my_chunk * 16 : reinterpret_cast<uint64_t>(p.k)), bytes);
+                const uint64_t v1 = shfl64(va, row);
+                cp_async16(at + KPW * ROW, reinterpret_cast<const void*>(bytes ? v1 + my_chunk * 16 : reinterpret_cast<uint64_t>(p.k)), bytes);
             }
             fetch();
         }
         cp_async_commit();
     };
+    // The queries of an item as the B operand, [k step][term][8 heads][lane]: a thread's entries are read from memory while the
+    // item before is joined, and stored when that is done.
+    float2 qx[SPLIT ? QN : 1][2];
+    uint2 qraw[SPLIT ? 1 : QN];
+    auto load_q = [&](uint32_t b, uint32_t h, uint32_t h0) {
+        const uint32_t heads = min((uint32_t)HEADS, p.group - h0);
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const uint32_t e = threadIdx.x + i * DEC_THREADS, ln = e % 32, nt = e / 32 % NT, ks = e / (32 * NT), head = nt * 8 + ln / 4, dim = ks * 16 + 2 * (ln % 4);
+            const int64_t at = (int64_t)b * p.q_row + (int64_t)(h * p.group + h0 + head) * p.q_head + dim;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool in = head < heads && dim + 8 * j < p.dim;
+                if constexpr (SPLIT) qx[i][j] = in ? *reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + at + 8 * j) : make_float2(0.f, 0.f);
+                else (j ? qraw[i].y : qraw[i].x) = in ? *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + at + 8 * j) : 0u;
+            }
+        }
+    };
+    auto store_q = [&]() {
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const uint32_t e = threadIdx.x + i * DEC_THREADS, ln = e % 32, nt = e / 32 % NT, ks = e / (32 * NT);
+            if constexpr (!SPLIT) {
+                qf[(ks * NT + nt) * 32 + ln] = qraw[i];
+            } else {  // the f32 value as a sum of 16-bit terms, each the rounding of what the ones before left
+                float2(&x)[2] = qx[i];
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) {
+                    const uint2 r = make_uint2(pack2<F16>(x[0].x, x[0].y), pack2<F16>(x[1].x, x[1].y));
+                    const float2 a = unpack2<F16>(r.x), c = unpack2<F16>(r.y);
+                    x[0].x -= a.x, x[0].y -= a.y, x[1].x -= c.x, x[1].y -= c.y;
+                    qf[((ks * TERMS + t) * NT + nt) * 32 + ln] = r;
+                }
+            }
+        }
+    };
+    load_q(c_b, c_h, c_h0);
     fetch();
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) issue(s);
 
     float o[KS][NT][4], m[NT][2], l[NT][2];
+    uint2 qr[Sh::Q_REGS ? KS * TERMS * NT : 1];
     bool fresh = true, begins = true;  // the next tile is the first of an item that this run sees; the run has the item's first tile
     uint32_t s = 0;
 #pragma unroll 1
@@ -240,37 +331,14 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
         cp_async_wait<STAGES - 1>();
         __syncwarp();
         const TileMeta mt = meta[s];
-        const uint32_t b = mt.b, h = mt.h, h0 = mt.h0, heads = min((uint32_t)HEADS, p.group - h0);
         if (fresh) {
             fresh = false;
             begins = mt.t == 0;
-            // the queries as the B operand, [k step][term][8 heads][lane]; every warp of the CTA has left the previous ones
-            for (uint32_t e = threadIdx.x; e < KS * NT * 32; e += DEC_THREADS) {
-                const uint32_t ln = e % 32, nt = e / 32 % NT, ks = e / (32 * NT), head = nt * 8 + ln / 4, dim = ks * 16 + 2 * (ln % 4);
-                float2 x[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                uint2 raw = make_uint2(0, 0);
-                const int64_t at = (int64_t)b * p.q_row + (int64_t)(h * p.group + h0 + head) * p.q_head + dim;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (head < heads && dim + 8 * j < p.dim) {
-                        if constexpr (SPLIT) x[j] = *reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + at + 8 * j);
-                        else (j ? raw.y : raw.x) = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + at + 8 * j);
-                    }
-                if constexpr (!SPLIT) {
-                    qf[(ks * NT + nt) * 32 + ln] = raw;
-                } else {  // the f32 value as a sum of 16-bit terms, each the rounding of what the ones before left
-#pragma unroll
-                    for (int t = 0; t < TERMS; ++t) {
-                        uint2 r;
-                        r.x = pack2<F16>(x[0].x, x[0].y);
-                        r.y = pack2<F16>(x[1].x, x[1].y);
-                        const float2 a = unpack2<F16>(r.x), c = unpack2<F16>(r.y);
-                        x[0].x -= a.x, x[0].y -= a.y, x[1].x -= c.x, x[1].y -= c.y;
-                        qf[((ks * TERMS + t) * NT + nt) * 32 + ln] = r;
-                    }
-                }
-            }
+            store_q();  // every warp has left the queries before these: it has passed the barrier that ends an item
             __syncthreads();
+            if constexpr (Sh::Q_REGS)
+#pragma unroll
+                for (int k = 0; k < KS * TERMS * NT; ++k) qr[k] = qf[k * 32 + lane];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 m[nt][0] = m[nt][1] = -INFINITY;
@@ -281,118 +349,133 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                     for (int c = 0; c < 4; ++c) o[k][nt][c] = 0.f;
             }
         }
-        const uint32_t kt = ring + s * Sh::STAGE, vt = kt + 16 * ROW;
+        const uint32_t kt = ring + s * Sh::STAGE, vt = kt + KPW * ROW;
         if (mt.valid > 0) {
-            // ---- scores: 16 keys x heads
-            // partial sums of each term, and of even and odd k steps: products that wait for one another cost more than the adds
-            constexpr int CH = NT == 1 && DP <= 128 ? 2 : 1;
-            float part[CH * TERMS][NT][4];
-#pragma unroll
-            for (int c = 0; c < CH * TERMS; ++c)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) part[c][nt][0] = part[c][nt][1] = part[c][nt][2] = part[c][nt][3] = 0.f;
+            // ---- scores: keys x heads.  Partial sums of each term, and of even and odd k steps where the registers last: products that
+            // wait for one another cost more than the adds
+            constexpr int CH = NT == 1 && MT == 1 && DP <= 128 ? 2 : 1;
+            float sc[MT][NT][4];
             {
+                float part[CH * TERMS][MT][NT][4];
+#pragma unroll
+                for (int c = 0; c < CH * TERMS; ++c)
+#pragma unroll
+                    for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) part[c][mi][nt][0] = part[c][mi][nt][1] = part[c][mi][nt][2] = part[c][mi][nt][3] = 0.f;
                 const uint32_t row = (lane & 7) + (lane & 8);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    uint32_t a[4];
-                    ldsm_x4(a, kt + row * ROW + (((2 * ks + (lane >> 4)) ^ (row & 7)) << 4));
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                    for (int t = 0; t < TERMS; ++t)
+                    for (int mi = 0; mi < MT; ++mi) {
+                        uint32_t a[4];
+                        ldsm_x4(a, kt + (16 * mi + row) * ROW + (((2 * ks + (lane >> 4)) ^ (row & 7)) << 4));
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const uint2 q = qf[((ks * TERMS + t) * NT + nt) * 32 + lane];
-                            mma16<F16>(part[CH * t + (ks & (CH - 1))][nt], a, q.x, q.y);
+                        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const int at = (ks * TERMS + t) * NT + nt;
+                                const uint2 q = Sh::Q_REGS ? qr[Sh::Q_REGS ? at : 0] : qf[at * 32 + lane];
+                                mma16<F16>(part[CH * t + (ks & (CH - 1))][mi][nt], a, q.x, q.y);
+                            }
+                    }
+#pragma unroll
+                for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float v = part[CH * TERMS - 1][mi][nt][c];
+#pragma unroll
+                            for (int t = CH * TERMS - 2; t >= 0; --t) v += part[t][mi][nt][c];  // the smallest terms first
+                            sc[mi][nt][c] = v;
                         }
-                }
             }
-            float sc[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    sc[nt][c] = 0.f;
-#pragma unroll
-                    for (int t = CH * TERMS - 1; t >= 0; --t) sc[nt][c] += part[t][nt][c];  // the smallest terms first
-                }
-            // ---- softmax: element c of a lane is key lane / 4 + 8 (c / 2), head 2 (lane % 4) + c % 2 of its eight
-            const bool in0 = (lane >> 2) < mt.valid, in1 = (lane >> 2) + 8 < mt.valid;
-            float alpha[NT][2];
-            uint32_t pt[TERMS][NT][2];  // the weights as a sum of 16-bit terms, too
+            // ---- softmax: element c of a lane is key 16 mi + lane / 4 + 8 (c / 2), head 2 (lane % 4) + c % 2 of its eight
+            uint32_t pt[TERMS][MT][NT][2];  // the weights as a sum of 16-bit terms, too
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float x[4];
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float mx = fmaxf(in0 ? sc[nt][c] * p.scale_log2 : -INFINITY, in1 ? sc[nt][c + 2] * p.scale_log2 : -INFINITY);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-                    mx = fmaxf(mx, m[nt][c]);
-                    alpha[nt][c] = mx == -INFINITY ? 1.f : exp2_approx(m[nt][c] - mx);
-                    m[nt][c] = mx;
-                    const float base = mx == -INFINITY ? 0.f : mx - WEIGHT_BIAS<F16>;
-                    x[c] = in0 ? exp2_approx(fmaf(sc[nt][c], p.scale_log2, -base)) : 0.f;
-                    x[c + 2] = in1 ? exp2_approx(fmaf(sc[nt][c + 2], p.scale_log2, -base)) : 0.f;
-                    l[nt][c] = fmaf(l[nt][c], alpha[nt][c], x[c] + x[c + 2]);
+                for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (16 * mi + (lane >> 2) + (c < 2 ? 0 : 8) >= mt.valid) sc[mi][nt][c] = -INFINITY;
+                        else sc[mi][nt][c] *= p.scale_log2;
+                        top[c & 1] = fmaxf(top[c & 1], sc[mi][nt][c]);
+                    }
+                if (__any_sync(0xFFFFFFFFu, top[0] > m[nt][0] + SLACK || top[1] > m[nt][1] + SLACK)) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = top[c];
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+                        mx = fmaxf(mx, m[nt][c]);
+                        const float alpha = mx == -INFINITY ? 1.f : exp2_approx(m[nt][c] - mx);
+                        m[nt][c] = mx;
+                        l[nt][c] *= alpha;
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) o[k][nt][c] *= alpha, o[k][nt][c + 2] *= alpha;
+                    }
                 }
+                const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0] - WEIGHT_BIAS<F16>, m[nt][1] == -INFINITY ? 0.f : m[nt][1] - WEIGHT_BIAS<F16>};
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int mi = 0; mi < MT; ++mi) {
+                    float x[4];
 #pragma unroll
-                    for (int t = 0; t < TERMS; ++t) {
-                        const uint32_t r = pack2<F16>(x[2 * j], x[2 * j + 1]);
-                        pt[t][nt][j] = transpose8(r);
-                        if constexpr (TERMS > 1) {
-                            const float2 a = unpack2<F16>(r);
-                            x[2 * j] -= a.x, x[2 * j + 1] -= a.y;
+                    for (int c = 0; c < 4; ++c) x[c] = exp2_approx(sc[mi][nt][c] - base[c & 1]);
+                    l[nt][0] += x[0] + x[2];
+                    l[nt][1] += x[1] + x[3];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int t = 0; t < TERMS; ++t) {
+                            const uint32_t r = pack2<F16>(x[2 * j], x[2 * j + 1]);
+                            pt[t][mi][nt][j] = transpose8(r);
+                            if constexpr (TERMS > 1) {
+                                const float2 a = unpack2<F16>(r);
+                                x[2 * j] -= a.x, x[2 * j + 1] -= a.y;
+                            }
                         }
-                    }
-                }
-                if constexpr (!SPLIT) {
-                    if (__any_sync(0xFFFFFFFFu, alpha[nt][0] != 1.f || alpha[nt][1] != 1.f)) {
-#pragma unroll
-                        for (int k = 0; k < KS; ++k)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) o[k][nt][c] *= alpha[nt][c & 1];
-                    }
                 }
             }
-            // ---- values: 16 elements of the head x heads, over the 16 keys
+            // ---- values: 16 elements of the head x heads, over the keys
             const uint32_t key = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                uint32_t a[4];
-                ldsm_x4_t(a, vt + key * ROW + (((2 * k + ((lane >> 3) & 1)) ^ (key & 7)) << 4));
+                uint32_t a[MT][4];
+#pragma unroll
+                for (int mi = 0; mi < MT; ++mi) ldsm_x4_t(a[mi], vt + (16 * mi + key) * ROW + (((2 * k + ((lane >> 3) & 1)) ^ (key & 7)) << 4));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     if constexpr (!SPLIT) {
-                        mma16<F16>(o[k][nt], a, pt[0][nt][0], pt[0][nt][1]);
+#pragma unroll
+                        for (int mi = 0; mi < MT; ++mi) mma16<F16>(o[k][nt], a[mi], pt[0][mi][nt][0], pt[0][mi][nt][1]);
                     } else {
                         // the tensor core cuts its sums off: over a long row that would show in an f32 result, so a tile is summed by
                         // itself, smallest terms first, and added with rounding
                         float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int t = TERMS - 1; t >= 0; --t) mma16<F16>(x, a, pt[t][nt][0], pt[t][nt][1]);
+                        for (int t = TERMS - 1; t >= 0; --t)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[k][nt][c] = fmaf(o[k][nt][c], alpha[nt][c & 1], x[c]);
+                            for (int mi = 0; mi < MT; ++mi) mma16<F16>(x, a[mi], pt[t][mi][nt][0], pt[t][mi][nt][1]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[k][nt][c] += x[c];
                     }
                 }
             }
         }
         if (mt.t + 1 == mt.nt || i + 1 == ntiles) {
             // ---- the item, or this run's part of it, is done: join the four warps
-            fresh = true;
+            const uint32_t b = mt.b, head0 = mt.h * p.group + mt.h0, heads = min((uint32_t)HEADS, p.group - mt.h0);
             const bool whole = begins && mt.t + 1 == mt.nt;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], 4);
-                    l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], 8);
-                    l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], 16);
-                    if (lane < 4) ml[warp * HEADS + nt * 8 + 2 * lane + c] = make_float2(m[nt][c], l[nt][c]);
-                }
-            __syncthreads();
+            fresh = true;
+            if (i + 1 < ntiles) {
+                const TileMeta nx = meta[s + 1 == STAGES ? 0 : s + 1];
+                load_q(nx.b, nx.h, nx.h0);
+            }
+            __syncwarp();
             // a warp's sums go to its part of the stage that it has just read, [head][DP], groups of eight elements swapped by head
             // so that neither the writes nor the reads of a warp meet in a bank
             float* mine = reinterpret_cast<float*>(smem + warp * Sh::WARP_STAGE + s * Sh::STAGE);
@@ -400,15 +483,15 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
+                    l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], 4);
+                    l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], 8);
+                    l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], 16);
                     const uint32_t head = nt * 8 + 2 * (lane & 3) + c;
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int w = 0; w < DEC_WARPS; ++w) mx = fmaxf(mx, ml[w * HEADS + head].x);
-                    const float f = m[nt][c] == -INFINITY ? 0.f : exp2_approx(m[nt][c] - mx);
+                    if (lane < 4) ml[warp * HEADS + head] = make_float2(m[nt][c], l[nt][c]);
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) mine[head * DP + ((k * 16 + j * 8 + (lane >> 2)) ^ ((lane & 3) << 3))] = o[k][nt][2 * j + c] * f;
+                        for (int j = 0; j < 2; ++j) mine[head * DP + ((k * 16 + j * 8 + (lane >> 2)) ^ ((lane & 3) << 3))] = o[k][nt][2 * j + c];
                 }
             __syncthreads();
             // the part of an item that begins before this run is the run's first, the part of one that ends behind it its last
@@ -424,63 +507,45 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
                 for (int w = 0; w < DEC_WARPS; ++w) {
                     const float4 x = *reinterpret_cast<const float4*>(from + w * Sh::WARP_STAGE);
                     const float2 y = ml[w * HEADS + head];
-                    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-                    if (y.x != -INFINITY) sum = fmaf(y.y, exp2_approx(y.x - mx), sum);
+                    const float f = y.x == -INFINITY ? 0.f : exp2_approx(y.x - mx);
+                    a.x = fmaf(x.x, f, a.x), a.y = fmaf(x.y, f, a.y), a.z = fmaf(x.z, f, a.z), a.w = fmaf(x.w, f, a.w);
+                    sum = fmaf(y.y, f, sum);
                 }
                 if (whole) {
-                    write_row<F16>(p, b, h * p.group + h0 + head, dim, a, mx, sum);
+                    write_row<F16>(p, b, head0 + head, dim, a, mx, sum);
                 } else {
                     *reinterpret_cast<float4*>(part + head * DP + dim) = a;
                     if (dim == 0) part[HEADS * DP + head] = mx, part[HEADS * DP + HEADS + head] = sum;
                 }
             }
+            __syncthreads();  // the parts are written; the stage and ml are free again
             if (!whole) {
-                // CTAs first .. last share the item; the one whose count completes theirs adds the parts in their order
-                const uint64_t g0 = begin + i - mt.t, g1 = g0 + mt.nt - 1;
-                const uint32_t first = (uint32_t)(((g0 + 1) * active - 1) / total), last = (uint32_t)(((g1 + 1) * active - 1) / total);
-                __threadfence();
-                __syncthreads();
-                if (threadIdx.x == 0) s_last = atomicAdd(d.counters + first, 1u) == last - first ? 1u : 0u;
-                __syncthreads();
-                if (s_last) {
-                    __threadfence();
-                    if (threadIdx.x == 0) d.counters[first] = 0;  // for the next call
-                    for (uint32_t e = threadIdx.x; e < heads * (DP / 4); e += DEC_THREADS) {
-                        const uint32_t head = e / (DP / 4), dim = 4 * (e % (DP / 4));
-                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                        float mx = -INFINITY, sum = 0.f;
-                        constexpr int AT_ONCE = 8;
-                        for (uint32_t c0 = first; c0 <= last; c0 += AT_ONCE) {
-                            float4 x[AT_ONCE];
-                            float pm[AT_ONCE], ps[AT_ONCE], top = mx;
-#pragma unroll
-                            for (int u = 0; u < AT_ONCE; ++u) {
-                                pm[u] = -INFINITY;
-                                if (c0 + u <= last) {
-                                    const float* q = d.part + (size_t)(2 * (c0 + u) + (c0 + u == first ? 1 : 0)) * Sh::PART;
-                                    x[u] = __ldcg(reinterpret_cast<const float4*>(q + head * DP + dim));
-                                    pm[u] = __ldcg(q + HEADS * DP + head);
-                                    ps[u] = __ldcg(q + HEADS * DP + HEADS + head);
-                                }
-                            }
-#pragma unroll
-                            for (int u = 0; u < AT_ONCE; ++u) top = fmaxf(top, pm[u]);
-                            const float f0 = mx == -INFINITY ? 0.f : exp2_approx(mx - top);
-                            a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0, sum *= f0;
-                            mx = top;
-#pragma unroll
-                            for (int u = 0; u < AT_ONCE; ++u)
-                                if (c0 + u <= last) {
-                                    const float f = pm[u] == -INFINITY ? 0.f : exp2_approx(pm[u] - top);
-                                    a.x = fmaf(x[u].x, f, a.x), a.y = fmaf(x[u].y, f, a.y), a.z = fmaf(x[u].z, f, a.z), a.w = fmaf(x[u].w, f, a.w);
-                                    sum = fmaf(ps[u], f, sum);
-                                }
-                        }
-                        write_row<F16>(p, b, h * p.group + h0 + head, dim, a, mx, sum);
+                // CTAs first .. last share the item; the one whose count completes theirs adds the parts in their order.  Within a run
+                // one warp sees to it while the others go on.
+                const bool at_end = i + 1 == ntiles;
+                if (at_end || warp == 0) {
+                    const uint64_t g0 = begin + i - mt.t, g1 = g0 + mt.nt - 1;
+                    const uint32_t first = (uint32_t)(((g0 + 1) * active - 1) / total), last = (uint32_t)(((g1 + 1) * active - 1) / total);
+                    uint32_t done = 0;
+                    if (threadIdx.x == 0) {
+                        __threadfence();  // the CTA's parts, which the barrier has shown to this thread, before the count
+                        done = atomicAdd(d.counters + first, 1u) == last - first ? 1u : 0u;
+                        __threadfence();
+                        if (done) d.counters[first] = 0;  // for the next call
+                        s_last = done;
                     }
+                    if (at_end) __syncthreads();
+                    done = at_end ? s_last : __shfl_sync(0xFFFFFFFFu, done, 0);
+                    if (done)
+                        for (uint32_t e = at_end ? threadIdx.x : lane; e < heads * (DP / 4); e += at_end ? DEC_THREADS : 32) {
+                            const uint32_t head = e / (DP / 4), dim = 4 * (e % (DP / 4));
+                            float4 a;
+                            float mx, sum;
+                            join_parts<HEADS, DP>(d.part, first, last, head, dim, a, mx, sum);
+                            write_row<F16>(p, b, head0 + head, dim, a, mx, sum);
+                        }
                 }
             }
-            __syncthreads();  // the stage, ml and s_last are free again
         }
         __syncwarp();
         issue(s);
@@ -491,8 +556,7 @@ __global__ void __launch_bounds__(DEC_THREADS, MINB) decode_kernel(const AttnPar
 template <int DP, int NT, bool F16, bool SPLIT>
 cudaError_t decode_go(const AttnParams& p, DecodePlan& d, uint32_t grid, cudaStream_t st) {
     using Sh = DecodeShape<DP, NT, F16, SPLIT>;
-    constexpr int MINB = DP == 64 ? 3 : DP == 128 ? 2 : 1;
-    auto kernel = decode_kernel<DP, NT, F16, SPLIT, MINB>;
+    auto kernel = decode_kernel<DP, NT, F16, SPLIT>;
     static PerDeviceOnce once;
     cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM); });
     if (e != cudaSuccess) return e;
@@ -508,7 +572,7 @@ cudaError_t decode_typed(const AttnParams& p, DecodePlan& d, uint32_t grid, cuda
 
 uint32_t padded_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 uint32_t head_tiles(uint32_t group) { return group > 8 ? 2 : 1; }
-uint32_t decode_grid(uint32_t dp, int sm_count) { return (uint32_t)sm_count * (dp == 64 ? 3 : dp == 128 ? 2 : 1); }
+uint32_t decode_grid(uint32_t dp, int sm_count) { return (uint32_t)sm_count * (dp <= 128 ? 2 : 1); }
 
 }  // namespace
 
@@ -526,7 +590,8 @@ cudaError_t launch_decode(const AttnParams& p, void* ws, int sm_count, cudaStrea
     d.counters = static_cast<uint32_t*>(ws);
     d.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + DEC_COUNTER_BYTES);
     // no more CTAs than tiles there can be
-    const uint64_t most = (uint64_t)p.requests * d.items * (((uint64_t)p.width * p.page.d + DEC_TILE - 1) / DEC_TILE);
+    const uint32_t tile = dp == 64 ? DecodeShape<64, 1, true, false>::TILE : DecodeShape<128, 1, true, false>::TILE;
+    const uint64_t most = (uint64_t)p.requests * d.items * (((uint64_t)p.width * p.page.d + tile - 1) / tile);
     uint32_t grid = decode_grid(dp, sm_count);
     if (grid > most) grid = (uint32_t)most;
     if (dp == 64) return nt == 1 ? decode_typed<64, 1>(p, d, grid, st) : decode_typed<64, 2>(p, d, grid, st);
