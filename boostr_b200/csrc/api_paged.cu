@@ -9,7 +9,7 @@ namespace b200q {
 size_t slots_max_requests();
 cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st);
 cudaError_t launch_rope(const RopeParams& p, int dtype, bool interleaved, uint32_t run, cudaStream_t st);
-cudaError_t launch_attn_rows(const AttnParams& p, cudaStream_t st);
+cudaError_t launch_prompt(const AttnParams& p, cudaStream_t st);
 size_t decode_workspace_bytes(uint32_t group, uint32_t dim, int sm_count);
 cudaError_t launch_decode(const AttnParams& p, void* ws, int sm_count, cudaStream_t st);
 }  // namespace b200q
@@ -69,7 +69,7 @@ int fill_attn(const char* op, AttnParams& p, const b200q_paged_cache* c, const v
     p.page.set((uint32_t)c->page_size);
     p.lens = lens, p.cu = nullptr, p.rows = (uint32_t)rows, p.requests = (uint32_t)requests;
     p.hq = (uint32_t)q_heads, p.hkv = (uint32_t)c->kv_heads, p.group = p.hq / p.hkv, p.dim = (uint32_t)c->head_dim;
-    p.scale_log2 = scale * 1.4426950408889634f;
+    p.scale_log2 = scale == 0.f ? 1e-30f : scale * 1.4426950408889634f;  // a factor that keeps minus infinity
     p.window = (uint32_t)window, p.sinks = (uint32_t)sinks;
     p.out = out, p.out_dtype = out_dtype, p.lse = lse;
     p.status = api_status();
@@ -175,7 +175,7 @@ int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t
                            scale, window, sinks, out, out_dtype, lse))
         return rc;
     p.cu = cu_seqlens;
-    return finish(op, launch_attn_rows(p, static_cast<cudaStream_t>(stream)));
+    return finish(op, launch_prompt(p, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -94,7 +94,7 @@ __device__ __forceinline__ uint32_t attn_len(const AttnParams& p, uint32_t b) {
 __device__ __forceinline__ bool attn_page(const AttnParams& p, uint32_t b, uint32_t j, uint32_t& page, uint32_t& tok) {
     const uint32_t e = p.page.div(j);
     tok = j - e * p.page.d;
-    page = (uint32_t)p.table[(int64_t)b * p.table_row + e];
+    page = e < p.width ? (uint32_t)p.table[(int64_t)b * p.table_row + e] : 0xFFFFFFFFu;
     if (page < p.pages) return true;
     atomicOr(p.status, STATUS_BAD_INDEX);
     return false;

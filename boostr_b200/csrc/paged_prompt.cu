@@ -1,0 +1,606 @@
+// Causal attention of the new tokens of prompts over a paged cache, on the 5th-generation tensor cores.
+//
+// A CTA owns two tiles of 128 query rows (one for heads over 128 wide).  A row is one query head of one token; all query heads
+// that share a key-value head stand next to one another, so a tile is 128 / group tokens and every key and value is read once for
+// all of them.  The keys that any row of the CTA sees (the sinks, then everything from the first row's window to the last
+// row's position) are numbered through without a gap and visited in tiles of 128.
+//
+//   scores   S = Q K^T: tcgen05.mma, Q and K in shared memory, S (f32) in tensor memory;
+//   softmax  one thread a row: reads its 128 scores, takes the weights P = 2^(s - m) against a maximum that follows the row only
+//            when a score exceeds it by 2^SLACK (then the row's sums are rescaled in tensor memory), writes P as 16-bit
+//            elements back to tensor memory;
+//   values   O += P V: P from tensor memory, V as it lies in shared memory (token rows, so the MMA reads it "MN-major").
+//
+// Warps 0-3 and 4-7 are the softmax of the two tiles, and while one works on its scores the tensor core has the other's products;
+// warps 8-11 bring the rows of the pages into a ring of swizzled tiles by 16-byte asynchronous copies (any page size, any
+// strides; rows that nobody sees are zeros, so nothing that lies in unused places reaches a sum); warp 12 issues the MMAs.
+// Bound: 4 flops for each visible pair and element on the tensor cores, and one exponential for each pair.
+// A product of a zero weight and a value that is not finite is not zero: rows that come out not finite are computed once more, key by key.
+#include "paged.cuh"
+#include "tcgen05_i8.cuh"
+
+namespace b200q {
+
+struct PromptPlan {
+    uint32_t heads;        // query heads of a tile: the group's, or 128 of them
+    uint32_t chunks;       // of the group
+    uint32_t tokens;       // of a tile: 128 / heads
+    uint32_t idesc_s, idesc_o;
+    uint32_t ksteps;       // of 16 elements of a head
+};
+
+namespace {
+
+constexpr float PR_SLACK = 5.f;
+template <bool F16>
+constexpr float PR_BIAS = F16 ? 9.f : 0.f;  // f16 weights are kept 2^9 times their size, their subnormals would lose the small ones
+
+constexpr int PR_THREADS = 512;
+constexpr int PR_LOADERS = 128;
+
+template <int DP>
+struct PromptShape {
+    static constexpr int NQ = DP == 256 ? 1 : 2;      // query tiles of a CTA
+    static constexpr int NK = DP == 256 ? 64 : 128;   // keys of a tile
+    static constexpr int SLOTS = DP == 64 ? 8 : 4;    // tiles of keys or values in the ring
+    static constexpr int Q_TILE = 128 * DP * 2, KV_TILE = NK * DP * 2;
+    static constexpr int OFF_Q = 0, OFF_KV = NQ * Q_TILE, OFF_ROWS = OFF_KV + SLOTS * KV_TILE, OFF_BAR = OFF_ROWS + 2 * 2 * 128 * 8,
+                         SMEM = OFF_BAR + 512 + 1024;  // 1 KB of slack for the alignment of the swizzled tiles
+    // tensor memory: scores, weights (over the scores where there is no room beside them), sums
+    static constexpr int COL_O = DP == 64 ? 256 : DP == 128 ? 256 : 128;
+    static constexpr bool P_OVER_S = DP == 128;
+    __host__ __device__ static constexpr int s_col(int t) { return t * NK; }
+    __host__ __device__ static constexpr int p_col(int t) { return P_OVER_S ? t * NK : DP == 64 ? 384 + 64 * t : 64; }
+    __host__ __device__ static constexpr int o_col(int t) { return COL_O + t * DP; }
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+                 "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D (128 x N, f32, tensor memory) (+)= A (128 x 16) B (16 x N); A in shared memory, or in tensor memory
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A 128-byte-swizzled tile of rows of 64 elements whose rows are the K dimension ("MN-major"): 8-row groups 1024 bytes apart,
+// blocks of 64 elements `block` bytes apart
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(((addr >> 4) & 0x3FFFu) | ((block >> 4) << 16)), "r"((1024u >> 4) | (1u << 14) | (2u << 29)));
+    return d;
+}
+
+// Waits and failures without calls: where the roles of a block hold different numbers of registers, calls cannot be compiled.
+__device__ __forceinline__ bool pr_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*dead || global_timer_ns() - t0 > 2000000000ull) return false;
+    }
+}
+// The same by a whole warp, with one answer for it.
+__device__ __forceinline__ bool pr_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* dead) {
+    return __all_sync(0xFFFFFFFFu, pr_wait(bar, parity, dead));
+}
+__device__ __forceinline__ void pr_fail(volatile uint32_t* dead, unsigned int* status, unsigned int code) {
+    if (!*dead) atomicOr(status, code);
+    *dead = 1;
+}
+
+// What a CTA works on.
+struct PromptWork {
+    uint32_t b, head, chunk;     // request, key-value head, chunk of its query heads
+    uint32_t row0, rows;         // first row of the CTA in q and its rows (tokens)
+    int64_t pos0;                // position of the first row (negative: before the request's first token)
+    uint32_t sinks, from, keys;  // visible keys: [0, sinks) and [from, from + keys - sinks)
+};
+
+// One row, key by key, by a whole warp (the plain form of the running softmax).
+__device__ __forceinline__ void prompt_row(const AttnParams& p, uint32_t b, uint32_t r, uint32_t h, int64_t pos) {
+    const uint32_t lane = threadIdx.x & 31;
+    const int64_t first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
+    const int dt = p.f16 ? DT_F16 : DT_BF16;
+    float q[8], o[8], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t e = 64 * (i / 2) + 2 * lane + i % 2;
+        q[i] = e < p.dim ? load_f32(p.q, (int64_t)r * p.q_row + (int64_t)h * p.q_head + e, p.q_dtype) * p.scale_log2 : 0.f;
+        o[i] = 0.f;
+    }
+    for (int64_t j = 0; j <= pos; ++j) {
+        if (j < first && j >= p.sinks) j = first;
+        uint32_t page, tok;
+        if (!attn_page(p, b, (uint32_t)j, page, tok)) continue;
+        const int64_t ka = (int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)(h / p.group) * p.k_head;
+        const int64_t va = (int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)(h / p.group) * p.v_head;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t e = 64 * (i / 2) + 2 * lane + i % 2;
+            if (e < p.dim) s = fmaf(q[i], load_f32(p.k, ka + e, dt), s);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+        const float m2 = fmaxf(m, s), c = m2 == -INFINITY ? 1.f : exp2f(m - m2), e2 = m2 == -INFINITY ? 0.f : exp2f(s - m2);
+        m = m2;
+        l = fmaf(l, c, e2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t e = 64 * (i / 2) + 2 * lane + i % 2;
+            if (e < p.dim) o[i] = fmaf(o[i], c, e2 * load_f32(p.v, va + e, dt));
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t e = 64 * (i / 2) + 2 * lane + i % 2;
+        if (e < p.dim) store_f32(p.out, ((int64_t)r * p.hq + h) * p.dim + e, p.out_dtype, o[i] * inv);
+    }
+    if (p.lse && lane == 0) p.lse[(int64_t)r * p.hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int DP, bool F16>
+__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptPlan d) {
+    using Sh = PromptShape<DP>;
+    constexpr int NQ = Sh::NQ, NK = Sh::NK, SLOTS = Sh::SLOTS;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const uint32_t bar = sbase + Sh::OFF_BAR;
+    const uint32_t bar_q = bar, bar_s = bar + 8, bar_p = bar + 24, bar_o = bar + 40, bar_full = bar + 64, bar_empty = bar + 64 + 8 * SLOTS;
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 256);
+    volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 260);
+    __shared__ uint32_t s_scan[PR_THREADS / 32], s_find[2];
+
+    grid_dep_wait();
+
+    // ---- which request and rows: CTAs over (pair of tiles, last first; key-value head), the heads of a pair next to one another
+    PromptWork w;
+    {
+        const uint32_t per = p.hkv * d.chunks, pair_rev = blockIdx.x / per, hc = blockIdx.x - pair_rev * per, step = NQ * d.tokens;
+        w.head = hc / d.chunks;
+        w.chunk = hc - w.head * d.chunks;
+        const uint32_t n = (p.requests + PR_THREADS - 1) / PR_THREADS;
+        const uint32_t b0 = min(p.requests, threadIdx.x * n), b1 = min(p.requests, b0 + n);
+        uint32_t sum = 0;
+        for (uint32_t b = b0; b < b1; ++b) sum += (uint32_t)(max(p.cu[b + 1] - p.cu[b], 0) + step - 1) / step;
+        uint32_t s = sum;
+#pragma unroll
+        for (int i = 1; i < 32; i *= 2) {
+            const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, s, i);
+            if (lane >= i) s += o;
+        }
+        if (lane == 31) s_scan[warp] = s;
+        __syncthreads();
+        uint32_t before = 0, total = 0;
+#pragma unroll
+        for (int i = 0; i < PR_THREADS / 32; ++i) {
+            if (i < warp) before += s_scan[i];
+            total += s_scan[i];
+        }
+        // rows behind the last request
+        const uint32_t used = (uint32_t)p.cu[p.requests];
+        for (uint32_t r = used + blockIdx.x; r < p.rows; r += gridDim.x) {
+            for (uint32_t i = threadIdx.x; i < p.hq * p.dim; i += PR_THREADS) store_f32(p.out, (int64_t)r * p.hq * p.dim + i, p.out_dtype, 0.f);
+            if (p.lse)
+                for (uint32_t i = threadIdx.x; i < p.hq; i += PR_THREADS) p.lse[(int64_t)r * p.hq + i] = -INFINITY;
+        }
+        if (pair_rev >= total) return;
+        const uint32_t pair = total - 1 - pair_rev;
+        uint32_t pre = before + s - sum;
+        if (pair >= pre && pair < pre + sum)
+            for (uint32_t b = b0; b < b1; ++b) {
+                const uint32_t t = (uint32_t)(max(p.cu[b + 1] - p.cu[b], 0) + step - 1) / step;
+                if (pair < pre + t) {
+                    s_find[0] = b;
+                    s_find[1] = (pair - pre) * step;
+                    break;
+                }
+                pre += t;
+            }
+        if (threadIdx.x == 0) {
+            mbar_init(bar_q, 4);
+            for (int t = 0; t < 2; ++t) {
+                mbar_init(bar_s + 8 * t, 1);
+                mbar_init(bar_p + 8 * t, 4);
+                mbar_init(bar_o + 8 * t, 1);
+            }
+            for (int i = 0; i < SLOTS; ++i) {
+                mbar_init(bar_full + 8 * i, 4);
+                mbar_init(bar_empty + 8 * i, 1);
+            }
+            *dead = 0;
+            mbar_fence_init();
+        }
+        if (warp == 12) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sbase + Sh::OFF_BAR + 256), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        tc_before();
+        __syncthreads();
+        tc_after();
+        grid_dep_launch();  // with the tensor memory in hand: a kernel behind this one may take some before it waits
+        w.b = s_find[0];
+        const uint32_t begin = (uint32_t)p.cu[w.b], end = min((uint32_t)p.cu[w.b + 1], p.rows), len = attn_len(p, w.b);
+        w.row0 = begin + s_find[1];
+        w.rows = w.row0 < end ? min(step, end - w.row0) : 0;
+        w.pos0 = (int64_t)len - (int64_t)p.cu[w.b + 1] + w.row0;
+        const int64_t last = w.pos0 + w.rows;  // one behind the last row's position
+        w.from = p.window && w.pos0 + 1 > (int64_t)p.window ? (uint32_t)(w.pos0 + 1 - p.window) : 0;
+        w.sinks = min(p.sinks, w.from);
+        w.keys = last > 0 && w.rows ? w.sinks + (uint32_t)last - w.from : 0;
+    }
+    const uint32_t tmem = *tmem_holder;
+    // rows, and tiles of keys, of each query tile; the last query tile has the most
+    const uint32_t nq = NQ == 2 && w.rows > d.tokens ? 2 : 1;
+    auto tiles_of = [&](uint32_t t) {
+        const int64_t end = w.pos0 + min(w.rows, (t + 1) * d.tokens);
+        return end > 0 && w.keys ? (w.sinks + (uint32_t)end - w.from + NK - 1) / NK : 0u;
+    };
+    const uint32_t n0 = tiles_of(0), nt = tiles_of(nq - 1);
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12 && nt) {
+            // -------------------------------------------------------------------------------------------- MMA issue
+            bool ok = pr_wait_warp(bar_q, 0, dead);
+            uint32_t pph[2] = {0, 0}, oph[2] = {0, 0};
+            auto slot_wait = [&](uint32_t item) {  // item 2 j: keys of tile j, 2 j + 1: values
+                if (ok && !pr_wait_warp(bar_full + 8 * (item % SLOTS), (item / SLOTS) & 1, dead)) ok = false;
+                tc_after();
+            };
+            auto scores = [&](uint32_t t, uint32_t item) {
+                const uint32_t q = sbase + Sh::OFF_Q + t * Sh::Q_TILE, k = sbase + Sh::OFF_KV + (item % SLOTS) * Sh::KV_TILE;
+                if (ok && elect_one_lane()) {
+#pragma unroll 4
+                    for (uint32_t i = 0; i < d.ksteps; ++i)
+                        tc_mma_ss(tmem + Sh::s_col(t), desc_sw128(desc_lo(q + (i >> 2) * (128 * 128) + (i & 3) * 32)),
+                                  desc_sw128(desc_lo(k + (i >> 2) * (NK * 128) + (i & 3) * 32)), d.idesc_s, i != 0);
+                    tc_commit_to(bar_s + 8 * t);
+                }
+                __syncwarp();
+            };
+            auto values = [&](uint32_t t, uint32_t item, bool accumulate) {
+                const uint32_t v = sbase + Sh::OFF_KV + (item % SLOTS) * Sh::KV_TILE;
+                if (ok && !pr_wait_warp(bar_p + 8 * t, pph[t], dead)) ok = false;
+                pph[t] ^= 1;
+                tc_after();
+                if (ok && elect_one_lane()) {
+#pragma unroll
+                    for (uint32_t i = 0; i < NK / 16; ++i)
+                        tc_mma_ts(tmem + Sh::o_col(t), tmem + Sh::p_col(t) + 8 * i, desc_mn(v + i * 2048, NK * 128), d.idesc_o, accumulate || i);
+                    tc_commit_to(bar_o + 8 * t);
+                }
+                __syncwarp();
+            };
+            auto release = [&](uint32_t item) {
+                if (ok && elect_one_lane()) tc_commit_to(bar_empty + 8 * (item % SLOTS));
+                __syncwarp();
+            };
+            slot_wait(0);
+            for (uint32_t t = 0; t < nq; ++t)
+                if (t == nq - 1 || n0) scores(t, 0);
+            release(0);
+            for (uint32_t j = 0; ok && j < nt; ++j) {
+                slot_wait(2 * j + 1);
+                bool have = false;
+#pragma unroll
+                for (uint32_t t = 0; t < 2; ++t) {
+                    if (t >= nq) continue;
+                    const uint32_t mine = t == nq - 1 ? nt : n0;
+                    if (j >= mine) continue;
+                    values(t, 2 * j + 1, j != 0);
+                    if (j + 1 < mine) {
+                        if (!have) slot_wait(2 * j + 2);
+                        have = true;
+                        // the next scores overwrite the weights that these products read
+                        if (Sh::P_OVER_S && ok && !pr_wait_warp(bar_o + 8 * t, oph[t], dead)) ok = false;
+                        scores(t, 2 * j + 2);
+                    }
+                    oph[t] ^= 1;
+                }
+                release(2 * j + 1);
+                if (j + 1 < nt) release(2 * j + 2);
+            }
+            // the last commit has arrived before the block ends (those before it then have, too)
+            if (ok) ok = pr_wait_warp(bar_empty + 8 * ((2 * nt - 1) % SLOTS), ((2 * nt - 1) / SLOTS) & 1, dead);
+            if (!ok && lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
+        }
+    } else if (warp >= 8) {
+        // ------------------------------------------------------------------------------------- rows into shared memory
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const uint32_t tid = threadIdx.x - 256;
+        constexpr uint32_t CPR = DP / 8;
+        uint64_t* rows = reinterpret_cast<uint64_t*>(smem + Sh::OFF_ROWS);  // [2 buffers][keys, values][128] addresses (0: zeros)
+        const uint32_t chunk = tid % CPR;
+        const bool in_dim = chunk * 8 < p.dim;
+        // a tile of `n` rows: 64-element blocks of [n][128 bytes], 16-byte chunks swizzled by the row
+        auto copy = [&](uint32_t dst, const uint64_t* from, uint32_t n) {
+            const uint32_t base = dst + (chunk >> 3) * (n * 128);
+#pragma unroll 8
+            for (uint32_t r = tid / CPR; r < n; r += PR_LOADERS / CPR) {
+                const uint64_t a = from[r];
+                const uint32_t bytes = a && in_dim ? 16 : 0;
+                cp_async16(base + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), reinterpret_cast<const void*>(bytes ? a + chunk * 16 : reinterpret_cast<uint64_t>(p.q)), bytes);
+            }
+            cp_async_commit();
+        };
+        bool ok = true;
+        if (nt) {
+            for (uint32_t t = 0; t < nq; ++t) {
+                const uint32_t tok = t * d.tokens + tid / d.heads, h = w.chunk * d.heads + tid % d.heads;
+                uint64_t a = 0;
+                if (tid < d.tokens * d.heads && tok < w.rows && h < p.group)
+                    a = reinterpret_cast<uint64_t>(p.q) + 2 * ((int64_t)(w.row0 + tok) * p.q_row + (int64_t)(w.head * p.group + h) * p.q_head);
+                rows[t * 256 + tid] = a;
+            }
+            named_bar_sync(1, PR_LOADERS);
+            for (uint32_t t = 0; t < nq; ++t) copy(sbase + Sh::OFF_Q + t * Sh::Q_TILE, rows + t * 256, 128);
+            named_bar_sync(1, PR_LOADERS);
+            // group 0 (and 1): the queries; then the items of the ring.  An item is announced when LAG younger ones are on their way, or
+            // before a wait.
+            constexpr uint32_t LAG = 2;
+            uint32_t announced = 0;  // items
+            bool q_announced = false;
+            auto announce = [&](uint32_t upto) {  // the caller has waited for the copies
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    if (!q_announced) mbar_arrive(bar_q);
+                    for (uint32_t i = announced; i < upto; ++i) mbar_arrive(bar_full + 8 * (i % SLOTS));
+                }
+                q_announced = true;
+                announced = upto;
+            };
+            for (uint32_t j = 0; j < nt; ++j) {  // to the end in any case: the loaders meet at barriers
+                uint64_t* at = rows + (j & 1) * 256;
+                const uint32_t v = j * NK + tid;
+                uint64_t ka = 0, va = 0;
+                if (tid < NK && v < w.keys) {
+                    const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
+                    uint32_t page, tok;
+                    if (attn_page(p, w.b, key, page, tok)) {
+                        ka = reinterpret_cast<uint64_t>(p.k) + 2 * ((int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)w.head * p.k_head);
+                        va = reinterpret_cast<uint64_t>(p.v) + 2 * ((int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)w.head * p.v_head);
+                    }
+                }
+                at[tid] = ka;
+                at[128 + tid] = va;
+                named_bar_sync(1, PR_LOADERS);
+#pragma unroll
+                for (uint32_t kv = 0; kv < 2; ++kv) {
+                    const uint32_t item = 2 * j + kv, slot = item % SLOTS;
+                    if (item >= SLOTS) {
+                        const uint32_t par = (item / SLOTS - 1) & 1;
+                        if (ok && !__all_sync(0xFFFFFFFFu, mbar_test(bar_empty + 8 * slot, par))) {
+                            cp_async_wait<0>();
+                            announce(item);
+                            ok = pr_wait_warp(bar_empty + 8 * slot, par, dead);
+                        }
+                    }
+                    // a CTA that gave up: the copies still end, into slots that nobody reads
+                    copy(sbase + Sh::OFF_KV + slot * Sh::KV_TILE, at + kv * 128, NK);
+                    if (item >= LAG && announced < item + 1 - LAG) {
+                        cp_async_wait<LAG>();
+                        announce(item + 1 - LAG);
+                    }
+                }
+            }
+            cp_async_wait<0>();
+            announce(2 * nt);
+            if (!ok && lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_EMPTY);
+        }
+    } else {
+        // ----------------------------------------------------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const uint32_t t = warp >> 2, r = (warp & 3) * 32 + lane;  // query tile, its row
+        const uint32_t tok = t * d.tokens + r / d.heads, h = w.chunk * d.heads + r % d.heads;
+        const bool live = t < nq && r < d.tokens * d.heads && tok < w.rows && h < p.group;
+        const int64_t pos = w.pos0 + tok;
+        // visible keys of the row by their number: [0, hi) but for [sinks, lo) (the first p.sinks keys have the first numbers, whether
+        // they lie before the CTA's window or in it)
+        const uint32_t hi = live && pos >= 0 ? w.sinks + (uint32_t)(pos + 1) - w.from : 0;
+        const uint32_t lo = p.window && pos + 1 > (int64_t)p.window ? w.sinks + (uint32_t)(pos + 1 - p.window) - w.from : w.sinks;
+        const uint32_t mine = t >= nq ? 0 : t == nq - 1 ? nt : n0;
+        const uint32_t lanes = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
+        const uint32_t s_at = lanes + Sh::s_col(t), p_at = lanes + Sh::p_col(t), o_at = lanes + Sh::o_col(t);
+        const float scale = fabsf(p.scale_log2);
+        float m = -INFINITY, l = 0.f;  // m: of the scaled scores
+        bool ok = true;
+        for (uint32_t j = 0; j < mine; ++j) {
+            if (!pr_wait_warp(bar_s + 8 * t, j & 1, dead)) {
+                ok = false;
+                break;
+            }
+            tc_after();
+            uint32_t s[NK / 32][32];
+#pragma unroll
+            for (int c = 0; c < NK / 32; ++c) tmem_ld32(s_at + 32 * c, s[c]);
+            tmem_ld_wait();
+            if (p.scale_log2 < 0.f)
+#pragma unroll
+                for (int c = 0; c < NK / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c][i] ^= 0x80000000u;
+            const uint32_t v0 = j * NK;
+            const bool cut = v0 + NK > hi || (lo > v0 && v0 + NK > p.sinks && lo > p.sinks);
+            if (__any_sync(0xFFFFFFFFu, cut)) {
+#pragma unroll
+                for (int c = 0; c < NK / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const uint32_t v = v0 + 32 * c + i;
+                        if (v >= hi || (v >= p.sinks && v < lo)) s[c][i] = 0xFF800000u;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < NK / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[c][i]));
+            mx *= scale;
+            const bool raise = mx > m + PR_SLACK;
+            if (__any_sync(0xFFFFFFFFu, raise)) {
+                const float top = raise ? mx : m, alpha = raise ? exp2_approx(m - mx) : 1.f;
+                m = top;
+                l *= alpha;
+                if (j) {
+                    if (!pr_wait_warp(bar_o + 8 * t, (j - 1) & 1, dead)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_after();
+#pragma unroll 1
+                    for (uint32_t c = 0; c < p.dim; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16_async(o_at + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st16_async(o_at + c, o);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : m - PR_BIAS<F16>;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NK / 32; ++c) {
+                uint32_t w16[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float a = exp2_approx(fmaf(__uint_as_float(s[c][2 * i]), scale, -base));
+                    const float b = exp2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), scale, -base));
+                    sum[(2 * i) & 3] += a;
+                    sum[(2 * i + 1) & 3] += b;
+                    w16[i] = pack2<F16>(a, b);
+                }
+                tmem_st16_async(p_at + 16 * c, w16);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p + 8 * t);
+        }
+        if (!ok && lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
+        // ---- the rows' sums
+        if (ok && mine) {
+            if (!pr_wait_warp(bar_o + 8 * t, (mine - 1) & 1, dead)) {
+                ok = false;
+                if (lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
+            }
+            tc_after();
+        }
+        if (t < nq && ok) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int64_t row = (int64_t)(w.row0 + tok) * p.hq + w.head * p.group + h;
+            float odd = 0.f;  // not zero: some element is not finite
+#pragma unroll 1
+            for (uint32_t c = 0; c < p.dim; c += 16) {
+                uint32_t o[16];
+                if (mine) {
+                    tmem_ld16_async(o_at + c, o);
+                    tmem_ld_wait();
+                }
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = hi ? __uint_as_float(o[i]) * inv : 0.f;
+                    if (c + i < p.dim) odd = fmaf(x[i], 0.f, odd);
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        if (c + i >= p.dim) break;
+                        if (p.out_dtype == DT_F32) {
+                            float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.dim + c + i);
+                            to[0] = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                            to[1] = make_float4(x[i + 4], x[i + 5], x[i + 6], x[i + 7]);
+                        } else {
+                            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.dim + c + i);
+                            *to = p.out_dtype == DT_F16
+                                      ? make_uint4(pack2<true>(x[i], x[i + 1]), pack2<true>(x[i + 2], x[i + 3]), pack2<true>(x[i + 4], x[i + 5]), pack2<true>(x[i + 6], x[i + 7]))
+                                      : make_uint4(pack2<false>(x[i], x[i + 1]), pack2<false>(x[i + 2], x[i + 3]), pack2<false>(x[i + 4], x[i + 5]), pack2<false>(x[i + 6], x[i + 7]));
+                        }
+                    }
+                }
+            }
+            if (live && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m - PR_BIAS<F16> + log2f(l)) * 0.6931471805599453f;
+            uint32_t again = __ballot_sync(0xFFFFFFFFu, live && odd != 0.f);
+            while (again) {
+                const int src = __ffs(again) - 1;
+                again &= again - 1;
+                const uint32_t r2 = __shfl_sync(0xFFFFFFFFu, w.row0 + tok, src), h2 = __shfl_sync(0xFFFFFFFFu, w.head * p.group + h, src);
+                prompt_row(p, w.b, r2, h2, w.pos0 + (int64_t)(r2 - w.row0));
+            }
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int DP, bool F16>
+cudaError_t prompt_go(const AttnParams& p, const PromptPlan& d, uint32_t grid, cudaStream_t st) {
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([] { return cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<DP>::SMEM); });
+    if (e != cudaSuccess) return e;
+    note_launch();
+    return launch_pdl(prompt_kernel<DP, F16>, dim3(grid), dim3(PR_THREADS), PromptShape<DP>::SMEM, st, p, d);
+}
+
+}  // namespace
+
+cudaError_t launch_prompt(const AttnParams& p, cudaStream_t st) {
+    PromptPlan d;
+    d.heads = p.group < 128 ? p.group : 128;
+    d.chunks = (p.group + d.heads - 1) / d.heads;
+    d.tokens = 128 / d.heads;
+    const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, nk = dp == 256 ? 64 : 128, nq = dp == 256 ? 1 : 2;
+    d.ksteps = (p.dim + 15) / 16;
+    const uint32_t type = p.f16 ? 0u : 1u, common = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);  // f32 sums, M = 128
+    d.idesc_s = common | ((nk >> 3) << 17);
+    d.idesc_o = common | (1u << 16) | ((d.ksteps * 16 >> 3) << 17);  // B: rows of tokens
+    // pairs of tiles there can be: whole ones, and one more at the end of each request
+    const uint32_t step = nq * d.tokens;
+    uint64_t pairs = (uint64_t)p.rows / step + p.requests;
+    if (pairs > p.rows) pairs = p.rows;
+    const uint64_t grid = pairs * p.hkv * d.chunks;
+    if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    if (dp == 64) return p.f16 ? prompt_go<64, true>(p, d, (uint32_t)grid, st) : prompt_go<64, false>(p, d, (uint32_t)grid, st);
+    if (dp == 128) return p.f16 ? prompt_go<128, true>(p, d, (uint32_t)grid, st) : prompt_go<128, false>(p, d, (uint32_t)grid, st);
+    return p.f16 ? prompt_go<256, true>(p, d, (uint32_t)grid, st) : prompt_go<256, false>(p, d, (uint32_t)grid, st);
+}
+
+}  // namespace b200q
