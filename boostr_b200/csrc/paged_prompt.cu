@@ -12,12 +12,14 @@
 //   values   O += P V: P from tensor memory, V as it lies in shared memory (token rows, so the MMA reads it "MN-major").
 //
 // Warps 0-3 and 4-7 are the softmax of the two tiles, and while one works on its scores the tensor core has the other's products;
-// warps 8-11 bring the rows of the pages into a ring of swizzled tiles by 16-byte asynchronous copies (any page size, any
-// strides; rows that nobody sees are zeros, so nothing that lies in unused places reaches a sum); warp 12 issues the MMAs.
+// warps 8-11 bring the rows of the pages into a ring of swizzled tiles: by TMA, a box for each run of up to 128 tokens inside
+// a page, or, where pages are no multiple of 8 tokens and in the last tile, by 16-byte asynchronous copies, which leave zeros where
+// there is no visible key (so nothing that lies in unused places reaches a sum); warp 12 issues the MMAs.
 // Bound: 4 flops for each visible pair and element on the tensor cores, and one exponential for each pair.
 // A product of a zero weight and a value that is not finite is not zero: rows that come out not finite are computed once more, key by key.
 #include "paged.cuh"
 #include "tcgen05_i8.cuh"
+#include "tmap.cuh"
 
 namespace b200q {
 
@@ -27,6 +29,7 @@ struct PromptPlan {
     uint32_t tokens;       // of a tile: 128 / heads
     uint32_t idesc_s, idesc_o;
     uint32_t ksteps;       // of 16 elements of a head
+    uint32_t rows;         // tokens of a TMA box: they lie in one page (0: no TMA)
 };
 
 namespace {
@@ -93,6 +96,13 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {
     uint64_t d;
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(((addr >> 4) & 0x3FFFu) | ((block >> 4) << 16)), "r"((1024u >> 4) | (1u << 14) | (2u << 29)));
     return d;
+}
+
+// Box {64 elements, 1 head, rows of a page, 1 page} of the cache; a page that does not exist reads as zeros
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t dim, uint32_t head, uint32_t tok, uint32_t page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+                 "r"(dim), "r"(head), "r"(tok), "r"(page), "r"(bar)
+                 : "memory");
 }
 
 // Waits and failures without calls: where the roles of a block hold different numbers of registers, calls cannot be compiled.
@@ -167,7 +177,8 @@ __device__ __forceinline__ void prompt_row(const AttnParams& p, uint32_t b, uint
 }
 
 template <int DP, bool F16>
-__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptPlan d) {
+__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptPlan d, const __grid_constant__ CUtensorMap map_k,
+                                                                const __grid_constant__ CUtensorMap map_v) {
     using Sh = PromptShape<DP>;
     constexpr int NQ = Sh::NQ, NK = Sh::NK, SLOTS = Sh::SLOTS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -254,8 +265,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         w.rows = w.row0 < end ? min(step, end - w.row0) : 0;
         w.pos0 = (int64_t)len - (int64_t)p.cu[w.b + 1] + w.row0;
         const int64_t last = w.pos0 + w.rows;  // one behind the last row's position
-        w.from = p.window && w.pos0 + 1 > (int64_t)p.window ? (uint32_t)(w.pos0 + 1 - p.window) : 0;
-        w.sinks = min(p.sinks, w.from);
+        // whole boxes: some keys more, which the rows' own limits hide
+        const uint32_t unit = d.rows ? d.rows : 1;
+        w.from = p.window && w.pos0 + 1 > (int64_t)p.window ? (uint32_t)(w.pos0 + 1 - p.window) / unit * unit : 0;
+        w.sinks = min((p.sinks + unit - 1) / unit * unit, w.from);
         w.keys = last > 0 && w.rows ? w.sinks + (uint32_t)last - w.from : 0;
     }
     const uint32_t tmem = *tmem_holder;
@@ -365,53 +378,74 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             named_bar_sync(1, PR_LOADERS);
             for (uint32_t t = 0; t < nq; ++t) copy(sbase + Sh::OFF_Q + t * Sh::Q_TILE, rows + t * 256, 128);
             named_bar_sync(1, PR_LOADERS);
-            // group 0 (and 1): the queries; then the items of the ring.  An item is announced when LAG younger ones are on their way, or
-            // before a wait.
+            // Whole tiles come by TMA where boxes fit into pages; the last tile, and other caches, by copies that fill the rows behind
+            // the last visible key with zeros.  A copied item is announced when LAG younger ones are on their way, or before a wait.
             constexpr uint32_t LAG = 2;
-            uint32_t announced = 0;  // items
-            bool q_announced = false;
-            auto announce = [&](uint32_t upto) {  // the caller has waited for the copies
+            const uint32_t whole = d.rows ? w.keys / NK : 0;  // tiles by TMA
+            const uint32_t blocks = (p.dim + 63) / 64, boxes = d.rows ? NK / d.rows * blocks : 0, lw = tid >> 5;
+            const uint32_t own = (boxes + 3 - lw) / 4;        // boxes of this warp: lw, lw + 4, ...
+            uint32_t announced = 2 * whole;                   // copied items
+            auto announce = [&](uint32_t upto) {              // the caller has waited for the copies
                 proxy_fence();
                 __syncwarp();
-                if (lane == 0) {
-                    if (!q_announced) mbar_arrive(bar_q);
+                if (lane == 0)
                     for (uint32_t i = announced; i < upto; ++i) mbar_arrive(bar_full + 8 * (i % SLOTS));
-                }
-                q_announced = true;
                 announced = upto;
             };
-            for (uint32_t j = 0; j < nt; ++j) {  // to the end in any case: the loaders meet at barriers
+            for (uint32_t item = 0; item < 2 * nt; ++item) {  // to the end in any case: the loaders meet at barriers
+                const uint32_t j = item >> 1, kv = item & 1, slot = item % SLOTS, dst = sbase + Sh::OFF_KV + slot * Sh::KV_TILE;
                 uint64_t* at = rows + (j & 1) * 256;
-                const uint32_t v = j * NK + tid;
-                uint64_t ka = 0, va = 0;
-                if (tid < NK && v < w.keys) {
-                    const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
-                    uint32_t page, tok;
-                    if (attn_page(p, w.b, key, page, tok)) {
-                        ka = reinterpret_cast<uint64_t>(p.k) + 2 * ((int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)w.head * p.k_head);
-                        va = reinterpret_cast<uint64_t>(p.v) + 2 * ((int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)w.head * p.v_head);
-                    }
-                }
-                at[tid] = ka;
-                at[128 + tid] = va;
-                named_bar_sync(1, PR_LOADERS);
-#pragma unroll
-                for (uint32_t kv = 0; kv < 2; ++kv) {
-                    const uint32_t item = 2 * j + kv, slot = item % SLOTS;
-                    if (item >= SLOTS) {
-                        const uint32_t par = (item / SLOTS - 1) & 1;
-                        if (ok && !__all_sync(0xFFFFFFFFu, mbar_test(bar_empty + 8 * slot, par))) {
-                            cp_async_wait<0>();
-                            announce(item);
-                            ok = pr_wait_warp(bar_empty + 8 * slot, par, dead);
+                if (j >= whole && !kv) {
+                    const uint32_t v = j * NK + tid;
+                    uint64_t ka = 0, va = 0;
+                    if (tid < NK && v < w.keys) {
+                        const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
+                        uint32_t page, tok;
+                        if (attn_page(p, w.b, key, page, tok)) {
+                            ka = reinterpret_cast<uint64_t>(p.k) + 2 * ((int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)w.head * p.k_head);
+                            va = reinterpret_cast<uint64_t>(p.v) + 2 * ((int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)w.head * p.v_head);
                         }
                     }
-                    // a CTA that gave up: the copies still end, into slots that nobody reads
-                    copy(sbase + Sh::OFF_KV + slot * Sh::KV_TILE, at + kv * 128, NK);
-                    if (item >= LAG && announced < item + 1 - LAG) {
-                        cp_async_wait<LAG>();
-                        announce(item + 1 - LAG);
+                    at[tid] = ka;
+                    at[128 + tid] = va;
+                    named_bar_sync(1, PR_LOADERS);
+                }
+                if (ok && item >= SLOTS) {
+                    const uint32_t par = (item / SLOTS - 1) & 1;
+                    if (!__all_sync(0xFFFFFFFFu, mbar_test(bar_empty + 8 * slot, par))) {
+                        if (announced < item) {
+                            cp_async_wait<0>();
+                            announce(item);
+                        }
+                        ok = pr_wait_warp(bar_empty + 8 * slot, par, dead);
                     }
+                }
+                if (j < whole) {
+                    if (ok) {
+                        if (lane == 0) mbar_expect_tx(bar_full + 8 * slot, own * d.rows * 128);
+                        __syncwarp();
+                        for (uint32_t i = lane; i < own; i += 32) {
+                            const uint32_t box = lw + 4 * i, g = box / blocks, blk = box - g * blocks, v = j * NK + g * d.rows;
+                            const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
+                            uint32_t page, tok;
+                            if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
+                            tma_rows(dst + blk * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * blk, w.head, tok, page, bar_full + 8 * slot);
+                        }
+                        __syncwarp();
+                    }
+                } else {  // a CTA that gave up: the copies still end, into slots that nobody reads
+                    copy(dst, at + kv * 128, NK);
+                    if (item + 1 >= announced + LAG) {
+                        cp_async_wait<LAG>();
+                        if (item + 1 - LAG > announced) announce(item + 1 - LAG);
+                    }
+                }
+                if (item == 1) {  // the queries, copied first
+                    cp_async_wait<0>();
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_q);
+                    if (!whole) announce(2);
                 }
             }
             cp_async_wait<0>();
@@ -461,12 +495,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                         if (v >= hi || (v >= p.sinks && v < lo)) s[c][i] = 0xFF800000u;
                     }
             }
-            float mx = -INFINITY;
+            float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < NK / 32; ++c)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[c][i]));
-            mx *= scale;
+                for (int i = 0; i < 32; i += 2)
+                    top4[(i >> 1) & 3] = fmaxf(fmaxf(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), top4[(i >> 1) & 3]);
+            const float mx = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
             const bool raise = mx > m + PR_SLACK;
             if (__any_sync(0xFFFFFFFFu, raise)) {
                 const float top = raise ? mx : m, alpha = raise ? exp2_approx(m - mx) : 1.f;
@@ -571,13 +606,31 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
     }
 }
 
+// The cache as a tensor of {elements, heads, tokens of a page, pages} in boxes of 64 elements and `rows` tokens; false: it cannot be one.
+bool cache_map(CUtensorMap* map, const void* base, bool f16, const AttnParams& p, int64_t page, int64_t tok, int64_t head, uint32_t rows) {
+    const EncodeTiledFn encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {p.dim, p.hkv, p.page.d, p.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)head * 2, (cuuint64_t)tok * 2, (cuuint64_t)page * 2};
+    const cuuint32_t box[4] = {64, 1, rows, 1}, one[4] = {1, 1, 1, 1};
+    return encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DP, bool F16>
-cudaError_t prompt_go(const AttnParams& p, const PromptPlan& d, uint32_t grid, cudaStream_t st) {
+cudaError_t prompt_go(const AttnParams& p, PromptPlan& d, uint32_t grid, cudaStream_t st) {
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<DP>::SMEM); });
     if (e != cudaSuccess) return e;
+    // the largest power of two that divides a page, if that is a whole swizzle pattern (8 rows)
+    CUtensorMap k = {}, v = {};
+    d.rows = p.page.d & (0u - p.page.d);
+    if (d.rows > (uint32_t)PromptShape<DP>::NK) d.rows = PromptShape<DP>::NK;
+    if (d.rows < 8 || !cache_map(&k, p.k, F16, p, p.k_page, p.k_tok, p.k_head, d.rows) || !cache_map(&v, p.v, F16, p, p.v_page, p.v_tok, p.v_head, d.rows))
+        d.rows = 0;
     note_launch();
-    return launch_pdl(prompt_kernel<DP, F16>, dim3(grid), dim3(PR_THREADS), PromptShape<DP>::SMEM, st, p, d);
+    return launch_pdl(prompt_kernel<DP, F16>, dim3(grid), dim3(PR_THREADS), PromptShape<DP>::SMEM, st, p, d, k, v);
 }
 
 }  // namespace
