@@ -29,7 +29,7 @@ struct PromptPlan {
     uint32_t tokens;       // of a tile: 128 / heads
     uint32_t idesc_s, idesc_o;
     uint32_t ksteps;       // of 16 elements of a head
-    uint32_t rows;         // tokens of a TMA box: they lie in one page (0: no TMA)
+    uint32_t rows;         // tokens of a TMA box of the cache: they lie in one page (0: no TMA)
 };
 
 namespace {
@@ -90,18 +90,17 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// A 128-byte-swizzled tile of rows of 64 elements whose rows are the K dimension ("MN-major"): 8-row groups 1024 bytes apart,
-// blocks of 64 elements `block` bytes apart
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(((addr >> 4) & 0x3FFFu) | ((block >> 4) << 16)), "r"((1024u >> 4) | (1u << 14) | (2u << 29)));
-    return d;
-}
-
 // Box {64 elements, 1 head, rows of a page, 1 page} of the cache; a page that does not exist reads as zeros
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t dim, uint32_t head, uint32_t tok, uint32_t page, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
                  "r"(dim), "r"(head), "r"(tok), "r"(page), "r"(bar)
+                 : "memory");
+}
+
+// Box {64 elements, heads of a tile, tokens of a tile} of the queries: the rows of a tile, in order
+__device__ __forceinline__ void tma_queries(uint32_t dst, const CUtensorMap* map, uint32_t dim, uint32_t head, uint32_t tok, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+                 "r"(dim), "r"(head), "r"(tok), "r"(bar)
                  : "memory");
 }
 
@@ -177,8 +176,8 @@ __device__ __forceinline__ void prompt_row(const AttnParams& p, uint32_t b, uint
 }
 
 template <int DP, bool F16>
-__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptPlan d, const __grid_constant__ CUtensorMap map_k,
-                                                                const __grid_constant__ CUtensorMap map_v) {
+__global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptPlan d, const __grid_constant__ CUtensorMap map_q,
+                                                                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using Sh = PromptShape<DP>;
     constexpr int NQ = Sh::NQ, NK = Sh::NK, SLOTS = Sh::SLOTS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -238,7 +237,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 pre += t;
             }
         if (threadIdx.x == 0) {
-            mbar_init(bar_q, 4);
+            mbar_init(bar_q, 1);
             for (int t = 0; t < 2; ++t) {
                 mbar_init(bar_s + 8 * t, 1);
                 mbar_init(bar_p + 8 * t, 4);
@@ -286,30 +285,36 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             // -------------------------------------------------------------------------------------------- MMA issue
             bool ok = pr_wait_warp(bar_q, 0, dead);
             uint32_t pph[2] = {0, 0}, oph[2] = {0, 0};
+            // descriptors by their low words: what changes from one product to the next is a sum, and the loops unroll
+            const uint32_t q_lo = desc_lo(sbase + Sh::OFF_Q), k_lo = desc_lo(sbase + Sh::OFF_KV);
+            const uint32_t v_lo = (((sbase + Sh::OFF_KV) >> 4) & 0x3FFFu) | (uint32_t)((NK * 128) >> 4) << 16;
             auto slot_wait = [&](uint32_t item) {  // item 2 j: keys of tile j, 2 j + 1: values
                 if (ok && !pr_wait_warp(bar_full + 8 * (item % SLOTS), (item / SLOTS) & 1, dead)) ok = false;
                 tc_after();
             };
             auto scores = [&](uint32_t t, uint32_t item) {
-                const uint32_t q = sbase + Sh::OFF_Q + t * Sh::Q_TILE, k = sbase + Sh::OFF_KV + (item % SLOTS) * Sh::KV_TILE;
+                const uint32_t q = q_lo + t * (Sh::Q_TILE >> 4), k = k_lo + (item % SLOTS) * (Sh::KV_TILE >> 4);
                 if (ok && elect_one_lane()) {
-#pragma unroll 4
-                    for (uint32_t i = 0; i < d.ksteps; ++i)
-                        tc_mma_ss(tmem + Sh::s_col(t), desc_sw128(desc_lo(q + (i >> 2) * (128 * 128) + (i & 3) * 32)),
-                                  desc_sw128(desc_lo(k + (i >> 2) * (NK * 128) + (i & 3) * 32)), d.idesc_s, i != 0);
+#pragma unroll
+                    for (uint32_t i = 0; i < DP / 16; ++i)
+                        if (i < d.ksteps)
+                            tc_mma_ss(tmem + Sh::s_col(t), desc_sw128(q + (i >> 2) * ((128 * 128) >> 4) + (i & 3) * 2),
+                                      desc_sw128(k + (i >> 2) * ((NK * 128) >> 4) + (i & 3) * 2), d.idesc_s, i != 0);
                     tc_commit_to(bar_s + 8 * t);
                 }
                 __syncwarp();
             };
+            // The values as they lie: rows of 64 elements are the K dimension ("MN-major"), 8-row groups 1024 bytes apart (the descriptor's
+            // stride), blocks of 64 elements NK * 128 bytes apart (its leading dimension)
             auto values = [&](uint32_t t, uint32_t item, bool accumulate) {
-                const uint32_t v = sbase + Sh::OFF_KV + (item % SLOTS) * Sh::KV_TILE;
+                const uint32_t v = v_lo + (item % SLOTS) * (Sh::KV_TILE >> 4);
                 if (ok && !pr_wait_warp(bar_p + 8 * t, pph[t], dead)) ok = false;
                 pph[t] ^= 1;
                 tc_after();
                 if (ok && elect_one_lane()) {
 #pragma unroll
                     for (uint32_t i = 0; i < NK / 16; ++i)
-                        tc_mma_ts(tmem + Sh::o_col(t), tmem + Sh::p_col(t) + 8 * i, desc_mn(v + i * 2048, NK * 128), d.idesc_o, accumulate || i);
+                        tc_mma_ts(tmem + Sh::o_col(t), tmem + Sh::p_col(t) + 8 * i, desc_sw128(v + i * (2048 >> 4)), d.idesc_o, accumulate || i);
                     tc_commit_to(bar_o + 8 * t);
                 }
                 __syncwarp();
@@ -368,21 +373,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         };
         bool ok = true;
         if (nt) {
-            for (uint32_t t = 0; t < nq; ++t) {
-                const uint32_t tok = t * d.tokens + tid / d.heads, h = w.chunk * d.heads + tid % d.heads;
-                uint64_t a = 0;
-                if (tid < d.tokens * d.heads && tok < w.rows && h < p.group)
-                    a = reinterpret_cast<uint64_t>(p.q) + 2 * ((int64_t)(w.row0 + tok) * p.q_row + (int64_t)(w.head * p.group + h) * p.q_head);
-                rows[t * 256 + tid] = a;
+            const uint32_t blocks = (p.dim + 63) / 64;
+            if (tid == 0) {  // rows behind the CTA's last, of other requests or heads, are computed and dropped
+                mbar_expect_tx(bar_q, nq * blocks * d.tokens * d.heads * 128);
+                for (uint32_t t = 0; t < nq; ++t)
+                    for (uint32_t b = 0; b < blocks; ++b)
+                        tma_queries(sbase + Sh::OFF_Q + t * Sh::Q_TILE + b * (128 * 128), &map_q, 64 * b, w.head * p.group + w.chunk * d.heads,
+                                    w.row0 + t * d.tokens, bar_q);
             }
-            named_bar_sync(1, PR_LOADERS);
-            for (uint32_t t = 0; t < nq; ++t) copy(sbase + Sh::OFF_Q + t * Sh::Q_TILE, rows + t * 256, 128);
-            named_bar_sync(1, PR_LOADERS);
+            __syncwarp();
             // Whole tiles come by TMA where boxes fit into pages; the last tile, and other caches, by copies that fill the rows behind
             // the last visible key with zeros.  A copied item is announced when LAG younger ones are on their way, or before a wait.
             constexpr uint32_t LAG = 2;
             const uint32_t whole = d.rows ? w.keys / NK : 0;  // tiles by TMA
-            const uint32_t blocks = (p.dim + 63) / 64, boxes = d.rows ? NK / d.rows * blocks : 0, lw = tid >> 5;
+            const uint32_t boxes = d.rows ? NK / d.rows * blocks : 0, lw = tid >> 5;
             const uint32_t own = (boxes + 3 - lw) / 4;        // boxes of this warp: lw, lw + 4, ...
             uint32_t announced = 2 * whole;                   // copied items
             auto announce = [&](uint32_t upto) {              // the caller has waited for the copies
@@ -440,13 +444,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                         if (item + 1 - LAG > announced) announce(item + 1 - LAG);
                     }
                 }
-                if (item == 1) {  // the queries, copied first
-                    cp_async_wait<0>();
-                    proxy_fence();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar_q);
-                    if (!whole) announce(2);
-                }
             }
             cp_async_wait<0>();
             announce(2 * nt);
@@ -461,8 +458,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         const int64_t pos = w.pos0 + tok;
         // visible keys of the row by their number: [0, hi) but for [sinks, lo) (the first p.sinks keys have the first numbers, whether
         // they lie before the CTA's window or in it)
-        const uint32_t hi = live && pos >= 0 ? w.sinks + (uint32_t)(pos + 1) - w.from : 0;
-        const uint32_t lo = p.window && pos + 1 > (int64_t)p.window ? w.sinks + (uint32_t)(pos + 1 - p.window) - w.from : w.sinks;
+        // rows that are dropped are not limited: limits cost
+        const uint32_t hi = !live ? 0xFFFFFFFFu : pos >= 0 ? w.sinks + (uint32_t)(pos + 1) - w.from : 0;
+        const uint32_t lo = live && p.window && pos + 1 > (int64_t)p.window ? w.sinks + (uint32_t)(pos + 1 - p.window) - w.from : w.sinks;
         const uint32_t mine = t >= nq ? 0 : t == nq - 1 ? nt : n0;
         const uint32_t lanes = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
         const uint32_t s_at = lanes + Sh::s_col(t), p_at = lanes + Sh::p_col(t), o_at = lanes + Sh::o_col(t);
@@ -558,35 +556,52 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int64_t row = (int64_t)(w.row0 + tok) * p.hq + w.head * p.group + h;
             float odd = 0.f;  // not zero: some element is not finite
+            // 16-bit results go through the rows of the query tile in shared memory, which nothing reads any more, so that a warp writes
+            // whole rows: 16-byte chunks, swapped by row against bank conflicts
+            uint8_t* stage = smem + Sh::OFF_Q + t * Sh::Q_TILE + (warp & 3) * (32 * DP * 2);
 #pragma unroll 1
-            for (uint32_t c = 0; c < p.dim; c += 16) {
-                uint32_t o[16];
+            for (uint32_t c = 0; c < p.dim; c += 32) {
+                uint32_t o[32];
                 if (mine) {
-                    tmem_ld16_async(o_at + c, o);
+                    tmem_ld32(o_at + c, o);
                     tmem_ld_wait();
                 }
-                float x[16];
+                float x[32];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[i] = hi ? __uint_as_float(o[i]) * inv : 0.f;
-                    if (c + i < p.dim) odd = fmaf(x[i], 0.f, odd);
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = hi && c + i < p.dim ? __uint_as_float(o[i]) * inv : 0.f;
+                    odd = fmaf(x[i], 0.f, odd);
                 }
-                if (live) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        if (c + i >= p.dim) break;
-                        if (p.out_dtype == DT_F32) {
+                for (int i = 0; i < 32; i += 8) {
+                    if (c + i >= p.dim) break;
+                    if (p.out_dtype == DT_F32) {
+                        if (live) {
                             float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.dim + c + i);
                             to[0] = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                             to[1] = make_float4(x[i + 4], x[i + 5], x[i + 6], x[i + 7]);
-                        } else {
-                            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.dim + c + i);
-                            *to = p.out_dtype == DT_F16
-                                      ? make_uint4(pack2<true>(x[i], x[i + 1]), pack2<true>(x[i + 2], x[i + 3]), pack2<true>(x[i + 4], x[i + 5]), pack2<true>(x[i + 6], x[i + 7]))
-                                      : make_uint4(pack2<false>(x[i], x[i + 1]), pack2<false>(x[i + 2], x[i + 3]), pack2<false>(x[i + 4], x[i + 5]), pack2<false>(x[i + 6], x[i + 7]));
                         }
+                    } else {
+                        *reinterpret_cast<uint4*>(stage + lane * (DP * 2) + ((((c + i) >> 3) ^ (lane & 7)) << 4)) =
+                            p.out_dtype == DT_F16
+                                ? make_uint4(pack2<true>(x[i], x[i + 1]), pack2<true>(x[i + 2], x[i + 3]), pack2<true>(x[i + 4], x[i + 5]), pack2<true>(x[i + 6], x[i + 7]))
+                                : make_uint4(pack2<false>(x[i], x[i + 1]), pack2<false>(x[i + 2], x[i + 3]), pack2<false>(x[i + 4], x[i + 5]), pack2<false>(x[i + 6], x[i + 7]));
                     }
                 }
+            }
+            __syncwarp();
+            if (p.out_dtype != DT_F32) {
+                constexpr uint32_t CPR = DP / 8;
+                const uint32_t all_live = __ballot_sync(0xFFFFFFFFu, live), chunk = lane % CPR;
+#pragma unroll 4
+                for (uint32_t q = 0; q < 32; q += 32 / CPR) {
+                    const uint32_t from = q + lane / CPR;
+                    const uint32_t to = __shfl_sync(0xFFFFFFFFu, (uint32_t)row, from);
+                    if ((all_live >> from & 1) && chunk * 8 < p.dim)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (int64_t)to * p.dim + chunk * 8) =
+                            *reinterpret_cast<const uint4*>(stage + from * (DP * 2) + ((chunk ^ (from & 7)) << 4));
+                }
+                __syncwarp();
             }
             if (live && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m - PR_BIAS<F16> + log2f(l)) * 0.6931471805599453f;
             uint32_t again = __ballot_sync(0xFFFFFFFFu, live && odd != 0.f);
@@ -618,19 +633,32 @@ bool cache_map(CUtensorMap* map, const void* base, bool f16, const AttnParams& p
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The queries as a tensor of {elements, heads, tokens} in boxes of a tile's rows.
+bool query_map(CUtensorMap* map, const AttnParams& p, const PromptPlan& d) {
+    const EncodeTiledFn encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {p.dim, p.hq, p.rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)p.q_head * 2, (cuuint64_t)p.q_row * 2};
+    const cuuint32_t box[3] = {64, d.heads, d.tokens}, one[3] = {1, 1, 1};
+    return encode(map, p.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p.q), dims, strides, box, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DP, bool F16>
 cudaError_t prompt_go(const AttnParams& p, PromptPlan& d, uint32_t grid, cudaStream_t st) {
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<DP>::SMEM); });
     if (e != cudaSuccess) return e;
     // the largest power of two that divides a page, if that is a whole swizzle pattern (8 rows)
-    CUtensorMap k = {}, v = {};
+    CUtensorMap q = {}, k = {}, v = {};
+    if (!query_map(&q, p, d)) return cudaErrorInvalidValue;
     d.rows = p.page.d & (0u - p.page.d);
     if (d.rows > (uint32_t)PromptShape<DP>::NK) d.rows = PromptShape<DP>::NK;
     if (d.rows < 8 || !cache_map(&k, p.k, F16, p, p.k_page, p.k_tok, p.k_head, d.rows) || !cache_map(&v, p.v, F16, p, p.v_page, p.v_tok, p.v_head, d.rows))
         d.rows = 0;
     note_launch();
-    return launch_pdl(prompt_kernel<DP, F16>, dim3(grid), dim3(PR_THREADS), PromptShape<DP>::SMEM, st, p, d, k, v);
+    return launch_pdl(prompt_kernel<DP, F16>, dim3(grid), dim3(PR_THREADS), PromptShape<DP>::SMEM, st, p, d, q, k, v);
 }
 
 }  // namespace
