@@ -38,24 +38,35 @@ constexpr float PR_SLACK = 5.f;
 template <bool F16>
 constexpr float PR_BIAS = F16 ? 9.f : 0.f;  // f16 weights are kept 2^9 times their size, their subnormals would lose the small ones
 
+// Of every eight pairs of weights, this many are computed by exp2_poly: the special-function unit takes 8 cycles for a warp's 32
+// exponentials, the cubic's instructions a good half of that.
+constexpr int PR_POLY = 2;
+
 constexpr int PR_THREADS = 512;
 constexpr int PR_LOADERS = 128;
 
+// Scores are read into registers at once, so their columns are free for the next scores while the weights are computed, and the
+// weights have columns of their own: 512 columns = 2 (NK scores + NK / 2 weights + DP sums) give 80 keys a tile at DP = 128.
+// (128 keys with the weights over the scores, where scores, softmax and values of a tile follow one another: 583 us for 8192 tokens,
+// 32 heads of 128.)
 template <int DP>
 struct PromptShape {
-    static constexpr int NQ = DP == 256 ? 1 : 2;      // query tiles of a CTA
-    static constexpr int NK = DP == 256 ? 64 : 128;   // keys of a tile
-    static constexpr int SLOTS = DP == 64 ? 8 : 4;    // tiles of keys or values in the ring
+    static constexpr int NQ = DP == 256 ? 1 : 2;                        // query tiles of a CTA
+    static constexpr int NK = DP == 256 ? 64 : DP == 128 ? 80 : 128;    // keys of a tile
+    static constexpr int SLOTS = DP == 64 ? 8 : DP == 128 ? 7 : 4;      // tiles of keys or values in the ring
     static constexpr int Q_TILE = 128 * DP * 2, KV_TILE = NK * DP * 2;
-    static constexpr int OFF_Q = 0, OFF_KV = NQ * Q_TILE, OFF_ROWS = OFF_KV + SLOTS * KV_TILE, OFF_BAR = OFF_ROWS + 2 * 2 * 128 * 8,
+    static constexpr int OFF_Q = 0, OFF_KV = NQ * Q_TILE, OFF_ROWS = OFF_KV + SLOTS * KV_TILE, OFF_BAR = OFF_ROWS + 3 * 2 * 128 * 8,
                          SMEM = OFF_BAR + 512 + 1024;  // 1 KB of slack for the alignment of the swizzled tiles
-    // tensor memory: scores, weights (over the scores where there is no room beside them), sums
-    static constexpr int COL_O = DP == 64 ? 256 : DP == 128 ? 256 : 128;
-    static constexpr bool P_OVER_S = DP == 128;
+    static_assert(KV_TILE % 1024 == 0 && SMEM <= 227 * 1024, "tiles of whole swizzle patterns that fit");
+    // tensor memory: scores, weights, sums
     __host__ __device__ static constexpr int s_col(int t) { return t * NK; }
-    __host__ __device__ static constexpr int p_col(int t) { return P_OVER_S ? t * NK : DP == 64 ? 384 + 64 * t : 64; }
-    __host__ __device__ static constexpr int o_col(int t) { return COL_O + t * DP; }
+    __host__ __device__ static constexpr int p_col(int t) { return NQ * NK + t * (NK / 2); }
+    __host__ __device__ static constexpr int o_col(int t) { return 512 - (NQ - t) * DP; }
+    static_assert(NQ * (NK + NK / 2 + DP) <= 512, "tensor memory");
 };
+// Items of the ring: K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1), as the products take them.
+__device__ __forceinline__ uint32_t item_k(uint32_t j) { return j ? 2 * j - 1 : 0; }
+__device__ __forceinline__ uint32_t item_v(uint32_t j, uint32_t n) { return j + 1 == n ? 2 * n - 1 : 2 * j + 2; }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -70,6 +81,11 @@ __device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
                  "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -90,6 +106,48 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Two f32 in a register pair: one instruction for both
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 f2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 f2_split(f32x2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ f32x2 f2_fma(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // a NaN among them wins
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two numbers up to 2^20 without the special-function unit: x = n + f with n the nearest integer (left in the low bits of
+// x + 1.5 2^23) and |f| <= 1/2, 2^f by a cubic (the one of smallest relative error, 1.02e-4, among those that are 1 at 0: integers
+// are exact, so that -127 and everything below gives 0), n added to the exponent.
+__device__ __forceinline__ float2 exp2_poly(f32x2 x) {
+    float2 c = f2_split(x);
+    x = f2(fmaxf(c.x, -127.f), fmaxf(c.y, -127.f));
+    const float magic = 12582912.f;
+    const f32x2 t = f2_add(x, f2(magic, magic)), n = f2_add(t, f2(-magic, -magic)), f = f2_fma(n, f2(-1.f, -1.f), x);
+    f32x2 y = f2_fma(f2(0.05500906f, 0.05500906f), f, f2(0.24221097f, 0.24221097f));
+    y = f2_fma(y, f, f2(0.6932829f, 0.6932829f));
+    y = f2_fma(y, f, f2(1.f, 1.f));
+    const float2 a = f2_split(y), b = f2_split(t);
+    return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(b.x) << 23)), __int_as_float(__float_as_int(a.y) + (__float_as_int(b.y) << 23)));
+}
+
 // Box {64 elements, 1 head, rows of a page, 1 page} of the cache; a page that does not exist reads as zeros
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t dim, uint32_t head, uint32_t tok, uint32_t page, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
@@ -185,7 +243,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
     const uint32_t sbase = smem_u32(smem);
     const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t bar = sbase + Sh::OFF_BAR;
-    const uint32_t bar_q = bar, bar_s = bar + 8, bar_p = bar + 24, bar_o = bar + 40, bar_full = bar + 64, bar_empty = bar + 64 + 8 * SLOTS;
+    // queries there; of a query tile: scores computed, scores read, weights written, values added; of a slot: filled, free
+    const uint32_t bar_q = bar, bar_s = bar + 8, bar_r = bar + 24, bar_p = bar + 40, bar_o = bar + 56, bar_full = bar + 80, bar_empty = bar + 80 + 8 * SLOTS;
     volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 256);
     volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 260);
     __shared__ uint32_t s_scan[PR_THREADS / 32], s_find[2];
@@ -240,11 +299,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             mbar_init(bar_q, 1);
             for (int t = 0; t < 2; ++t) {
                 mbar_init(bar_s + 8 * t, 1);
+                mbar_init(bar_r + 8 * t, 4);
                 mbar_init(bar_p + 8 * t, 4);
                 mbar_init(bar_o + 8 * t, 1);
             }
             for (int i = 0; i < SLOTS; ++i) {
-                mbar_init(bar_full + 8 * i, 4);
+                mbar_init(bar_full + 8 * i, 1);
                 mbar_init(bar_empty + 8 * i, 1);
             }
             *dead = 0;
@@ -281,83 +341,99 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12 && nt) {
+        if (warp == 12 && nt && elect_one_lane()) {
             // -------------------------------------------------------------------------------------------- MMA issue
-            bool ok = pr_wait_warp(bar_q, 0, dead);
-            uint32_t pph[2] = {0, 0}, oph[2] = {0, 0};
-            // descriptors by their low words: what changes from one product to the next is a sum, and the loops unroll
+            // One thread: what it does between two products is time in which the tensor core may run dry.  Descriptors by their low
+            // words, so that what changes from one product to the next is a sum.
             const uint32_t q_lo = desc_lo(sbase + Sh::OFF_Q), k_lo = desc_lo(sbase + Sh::OFF_KV);
             const uint32_t v_lo = (((sbase + Sh::OFF_KV) >> 4) & 0x3FFFu) | (uint32_t)((NK * 128) >> 4) << 16;
-            auto slot_wait = [&](uint32_t item) {  // item 2 j: keys of tile j, 2 j + 1: values
-                if (ok && !pr_wait_warp(bar_full + 8 * (item % SLOTS), (item / SLOTS) & 1, dead)) ok = false;
+            bool ok = true;
+            auto wait = [&](uint32_t b, uint32_t phase) {
+                if (ok && !pr_wait(b, phase & 1, dead)) ok = false;
                 tc_after();
             };
-            auto scores = [&](uint32_t t, uint32_t item) {
-                const uint32_t q = q_lo + t * (Sh::Q_TILE >> 4), k = k_lo + (item % SLOTS) * (Sh::KV_TILE >> 4);
-                if (ok && elect_one_lane()) {
+            auto scores = [&](uint32_t t, uint32_t slot) {
+                if (!ok) return;
+                const uint32_t q = q_lo + t * (Sh::Q_TILE >> 4), k = k_lo + slot * (Sh::KV_TILE >> 4);
+                auto product = [&](uint32_t i) {
+                    tc_mma_ss(tmem + Sh::s_col(t), desc_sw128(q + (i >> 2) * ((128 * 128) >> 4) + (i & 3) * 2),
+                              desc_sw128(k + (i >> 2) * ((NK * 128) >> 4) + (i & 3) * 2), d.idesc_s, i != 0);
+                };
+                if (d.ksteps == DP / 16) {
 #pragma unroll
-                    for (uint32_t i = 0; i < DP / 16; ++i)
-                        if (i < d.ksteps)
-                            tc_mma_ss(tmem + Sh::s_col(t), desc_sw128(q + (i >> 2) * ((128 * 128) >> 4) + (i & 3) * 2),
-                                      desc_sw128(k + (i >> 2) * ((NK * 128) >> 4) + (i & 3) * 2), d.idesc_s, i != 0);
-                    tc_commit_to(bar_s + 8 * t);
+                    for (uint32_t i = 0; i < DP / 16; ++i) product(i);
+                } else {
+#pragma unroll 1
+                    for (uint32_t i = 0; i < d.ksteps; ++i) product(i);
                 }
-                __syncwarp();
+                tc_commit_to(bar_s + 8 * t);
             };
             // The values as they lie: rows of 64 elements are the K dimension ("MN-major"), 8-row groups 1024 bytes apart (the descriptor's
             // stride), blocks of 64 elements NK * 128 bytes apart (its leading dimension)
-            auto values = [&](uint32_t t, uint32_t item, bool accumulate) {
-                const uint32_t v = v_lo + (item % SLOTS) * (Sh::KV_TILE >> 4);
-                if (ok && !pr_wait_warp(bar_p + 8 * t, pph[t], dead)) ok = false;
-                pph[t] ^= 1;
-                tc_after();
-                if (ok && elect_one_lane()) {
+            auto values = [&](uint32_t t, uint32_t slot, bool accumulate) {
+                if (!ok) return;
+                const uint32_t v = v_lo + slot * (Sh::KV_TILE >> 4);
 #pragma unroll
-                    for (uint32_t i = 0; i < NK / 16; ++i)
-                        tc_mma_ts(tmem + Sh::o_col(t), tmem + Sh::p_col(t) + 8 * i, desc_sw128(v + i * (2048 >> 4)), d.idesc_o, accumulate || i);
-                    tc_commit_to(bar_o + 8 * t);
-                }
-                __syncwarp();
+                for (uint32_t i = 0; i < NK / 16; ++i)
+                    tc_mma_ts(tmem + Sh::o_col(t), tmem + Sh::p_col(t) + 8 * i, desc_sw128(v + i * (2048 >> 4)), d.idesc_o, accumulate || i);
+                tc_commit_to(bar_o + 8 * t);
             };
-            auto release = [&](uint32_t item) {
-                if (ok && elect_one_lane()) tc_commit_to(bar_empty + 8 * (item % SLOTS));
-                __syncwarp();
+            // the items of the ring in their order: the current one's slot and phase
+            uint32_t slot = 0, phase = 0;
+            auto advance = [&]() {
+                if (ok) tc_commit_to(bar_empty + 8 * slot);  // free when the products so far are done
+                if (++slot == SLOTS) slot = 0, phase ^= 1;
             };
-            slot_wait(0);
-            for (uint32_t t = 0; t < nq; ++t)
-                if (t == nq - 1 || n0) scores(t, 0);
-            release(0);
-            for (uint32_t j = 0; ok && j < nt; ++j) {
-                slot_wait(2 * j + 1);
-                bool have = false;
+            wait(bar_q, 0);
+            // While a tile's weights are computed, its next scores are, too; the products of the two tiles alternate.
+            wait(bar_full, 0);
 #pragma unroll
-                for (uint32_t t = 0; t < 2; ++t) {
-                    if (t >= nq) continue;
-                    const uint32_t mine = t == nq - 1 ? nt : n0;
-                    if (j >= mine) continue;
-                    values(t, 2 * j + 1, j != 0);
-                    if (j + 1 < mine) {
-                        if (!have) slot_wait(2 * j + 2);
-                        have = true;
-                        // the next scores overwrite the weights that these products read
-                        if (Sh::P_OVER_S && ok && !pr_wait_warp(bar_o + 8 * t, oph[t], dead)) ok = false;
-                        scores(t, 2 * j + 2);
+            for (uint32_t t = 0; t < NQ; ++t)
+                if (t < nq && (t == nq - 1 ? nt : n0) > 0) scores(t, 0);
+            advance();
+            if (nt > 1) {
+                wait(bar_full + 8 * slot, phase);
+#pragma unroll
+                for (uint32_t t = 0; t < NQ; ++t)
+                    if (t < nq && (t == nq - 1 ? nt : n0) > 1) {
+                        wait(bar_r + 8 * t, 0);
+                        scores(t, slot);
                     }
-                    oph[t] ^= 1;
+                advance();
+            }
+            for (uint32_t j = 0; ok && j < nt; ++j) {
+                // values of tile j in this slot, keys of tile j + 2 in the next
+                const uint32_t next = slot + 1 == SLOTS ? 0 : slot + 1, next_phase = slot + 1 == SLOTS ? phase ^ 1 : phase;
+                bool have_v = false, have_k = false;
+#pragma unroll
+                for (uint32_t t = 0; t < NQ; ++t) {
+                    const uint32_t mine = t == nq - 1 ? nt : n0;
+                    if (t >= nq || j >= mine) continue;
+                    if (!have_v) wait(bar_full + 8 * slot, phase);
+                    have_v = true;
+                    wait(bar_p + 8 * t, j);
+                    values(t, slot, j != 0);
+                    if (j + 2 < mine) {
+                        if (!have_k) wait(bar_full + 8 * next, next_phase);
+                        have_k = true;
+                        wait(bar_r + 8 * t, j + 1);
+                        scores(t, next);
+                    }
                 }
-                release(2 * j + 1);
-                if (j + 1 < nt) release(2 * j + 2);
+                advance();
+                if (j + 2 < nt) advance();
             }
             // the last commit has arrived before the block ends (those before it then have, too)
-            if (ok) ok = pr_wait_warp(bar_empty + 8 * ((2 * nt - 1) % SLOTS), ((2 * nt - 1) / SLOTS) & 1, dead);
-            if (!ok && lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
+            if (ok) ok = pr_wait(bar_empty + 8 * ((2 * nt - 1) % SLOTS), ((2 * nt - 1) / SLOTS) & 1, dead);
+            if (!ok) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
         }
+        __syncwarp();
     } else if (warp >= 8) {
         // ------------------------------------------------------------------------------------- rows into shared memory
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const uint32_t tid = threadIdx.x - 256;
         constexpr uint32_t CPR = DP / 8;
-        uint64_t* rows = reinterpret_cast<uint64_t*>(smem + Sh::OFF_ROWS);  // [2 buffers][keys, values][128] addresses (0: zeros)
+        uint64_t* rows = reinterpret_cast<uint64_t*>(smem + Sh::OFF_ROWS);  // [3 buffers][keys, values][128] addresses (0: zeros)
         const uint32_t chunk = tid % CPR;
         const bool in_dim = chunk * 8 < p.dim;
         // a tile of `n` rows: 64-element blocks of [n][128 bytes], 16-byte chunks swizzled by the row
@@ -382,71 +458,80 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                                     w.row0 + t * d.tokens, bar_q);
             }
             __syncwarp();
-            // Whole tiles come by TMA where boxes fit into pages; the last tile, and other caches, by copies that fill the rows behind
-            // the last visible key with zeros.  A copied item is announced when LAG younger ones are on their way, or before a wait.
-            constexpr uint32_t LAG = 2;
-            const uint32_t whole = d.rows ? w.keys / NK : 0;  // tiles by TMA
-            const uint32_t boxes = d.rows ? NK / d.rows * blocks : 0, lw = tid >> 5;
-            const uint32_t own = (boxes + 3 - lw) / 4;        // boxes of this warp: lw, lw + 4, ...
-            uint32_t announced = 2 * whole;                   // copied items
-            auto announce = [&](uint32_t upto) {              // the caller has waited for the copies
-                proxy_fence();
-                __syncwarp();
-                if (lane == 0)
-                    for (uint32_t i = announced; i < upto; ++i) mbar_arrive(bar_full + 8 * (i % SLOTS));
-                announced = upto;
-            };
-            for (uint32_t item = 0; item < 2 * nt; ++item) {  // to the end in any case: the loaders meet at barriers
-                const uint32_t j = item >> 1, kv = item & 1, slot = item % SLOTS, dst = sbase + Sh::OFF_KV + slot * Sh::KV_TILE;
-                uint64_t* at = rows + (j & 1) * 256;
-                if (j >= whole && !kv) {
-                    const uint32_t v = j * NK + tid;
-                    uint64_t ka = 0, va = 0;
-                    if (tid < NK && v < w.keys) {
-                        const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
-                        uint32_t page, tok;
-                        if (attn_page(p, w.b, key, page, tok)) {
-                            ka = reinterpret_cast<uint64_t>(p.k) + 2 * ((int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)w.head * p.k_head);
-                            va = reinterpret_cast<uint64_t>(p.v) + 2 * ((int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)w.head * p.v_head);
-                        }
-                    }
-                    at[tid] = ka;
-                    at[128 + tid] = va;
-                    named_bar_sync(1, PR_LOADERS);
-                }
-                if (ok && item >= SLOTS) {
-                    const uint32_t par = (item / SLOTS - 1) & 1;
-                    if (!__all_sync(0xFFFFFFFFu, mbar_test(bar_empty + 8 * slot, par))) {
-                        if (announced < item) {
-                            cp_async_wait<0>();
-                            announce(item);
-                        }
-                        ok = pr_wait_warp(bar_empty + 8 * slot, par, dead);
-                    }
-                }
-                if (j < whole) {
-                    if (ok) {
-                        if (lane == 0) mbar_expect_tx(bar_full + 8 * slot, own * d.rows * 128);
-                        __syncwarp();
-                        for (uint32_t i = lane; i < own; i += 32) {
-                            const uint32_t box = lw + 4 * i, g = box / blocks, blk = box - g * blocks, v = j * NK + g * d.rows;
-                            const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
-                            uint32_t page, tok;
+            // Whole tiles come by TMA where boxes fit into pages: the warps take the items in turn, a lane finds the pages of a box, one
+            // lane issues them all.
+            const uint32_t whole = d.rows ? w.keys / NK : 0, lw = tid >> 5;  // tiles by TMA
+            if (whole) {
+                const uint32_t groups = NK / d.rows, last = whole == nt ? 2 * nt : 2 * nt - 1;
+                uint32_t slot = lw, par = 1;  // par: of the slot's last release; the first round waits for nothing
+                for (uint32_t item = lw; ok && item < last; item += 4) {
+                    const uint32_t kv = item + 1 == 2 * nt || (item && !(item & 1)), j = item + 1 == 2 * nt ? nt - 1 : kv ? item / 2 - 1 : (item + 1) / 2;
+                    if (j < whole) {
+                        uint32_t page = 0, tok = 0;
+                        if (lane < groups) {
+                            const uint32_t v = j * NK + lane * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
                             if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
-                            tma_rows(dst + blk * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * blk, w.head, tok, page, bar_full + 8 * slot);
+                        }
+                        if (item >= SLOTS) ok = pr_wait_warp(bar_empty + 8 * slot, par, dead);
+                        const uint32_t dst = sbase + Sh::OFF_KV + slot * Sh::KV_TILE, full = bar_full + 8 * slot;
+                        if (ok && lane == 0) mbar_expect_tx(full, groups * blocks * d.rows * 128);
+                        for (uint32_t g = 0; g < groups; ++g) {
+                            const uint32_t pg = __shfl_sync(0xFFFFFFFFu, page, g), tk = __shfl_sync(0xFFFFFFFFu, tok, g);
+                            if (ok && lane == 0)
+                                for (uint32_t b = 0; b < blocks; ++b)
+                                    tma_rows(dst + b * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * b, w.head, tk, pg, full);
                         }
                         __syncwarp();
                     }
-                } else {  // a CTA that gave up: the copies still end, into slots that nobody reads
-                    copy(dst, at + kv * 128, NK);
-                    if (item + 1 >= announced + LAG) {
+                    slot += 4;
+                    if (slot >= SLOTS) slot -= SLOTS, par ^= 1;
+                }
+            }
+            // Other caches, and the last tile: by copies that fill the rows behind the last visible key with zeros.  An item is announced
+            // when LAG younger ones are on their way.  (A slot is free when the item in it and the one behind that have been used, and
+            // those were announced long before the slot comes round: SLOTS > LAG + 1.)
+            constexpr uint32_t LAG = 2;
+            uint32_t copied = 0, told = 0;
+            auto announce = [&](uint32_t upto) {  // the caller has waited for its own copies
+                proxy_fence();
+                named_bar_sync(1, PR_LOADERS);
+                if (tid == 0)
+                    for (uint32_t i = told; i < upto; ++i) {
+                        const uint32_t item = !whole ? i : i ? 2 * nt - 1 : item_k(nt - 1);
+                        mbar_arrive(bar_full + 8 * (item % SLOTS));
+                    }
+                told = upto;
+            };
+            for (uint32_t j = whole; j < nt; ++j) {  // to the end in any case: the loaders meet at barriers
+                uint64_t* at = rows + j % 3 * 256;   // a third one is written while the slowest thread reads the first
+                const uint32_t v = j * NK + tid;
+                uint64_t ka = 0, va = 0;
+                if (tid < NK && v < w.keys) {
+                    const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
+                    uint32_t page, tok;
+                    if (attn_page(p, w.b, key, page, tok)) {
+                        ka = reinterpret_cast<uint64_t>(p.k) + 2 * ((int64_t)page * p.k_page + (int64_t)tok * p.k_tok + (int64_t)w.head * p.k_head);
+                        va = reinterpret_cast<uint64_t>(p.v) + 2 * ((int64_t)page * p.v_page + (int64_t)tok * p.v_tok + (int64_t)w.head * p.v_head);
+                    }
+                }
+                at[tid] = ka;
+                at[128 + tid] = va;
+                named_bar_sync(1, PR_LOADERS);
+                // keys of tile j, then values of the tile before (and, behind the last keys, of the last one)
+                for (uint32_t k = 0; k < 3; ++k) {
+                    if ((k == 1 && j == whole) || (k == 2 && j + 1 < nt)) continue;
+                    const uint32_t of = k == 1 ? j - 1 : j, item = k ? item_v(of, nt) : item_k(of), slot = item % SLOTS;
+                    if (ok && item >= SLOTS) ok = pr_wait_warp(bar_empty + 8 * slot, (item / SLOTS - 1) & 1, dead);
+                    // a CTA that gave up: the copies still end, into slots that nobody reads
+                    copy(sbase + Sh::OFF_KV + slot * Sh::KV_TILE, rows + of % 3 * 256 + (k ? 128 : 0), NK);
+                    if (++copied > told + LAG) {
                         cp_async_wait<LAG>();
-                        if (item + 1 - LAG > announced) announce(item + 1 - LAG);
+                        announce(copied - LAG);
                     }
                 }
             }
             cp_async_wait<0>();
-            announce(2 * nt);
+            if (told < copied) announce(copied);
             if (!ok && lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_EMPTY);
         }
     } else {
@@ -473,36 +558,47 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 break;
             }
             tc_after();
-            uint32_t s[NK / 32][32];
+            uint32_t s[NK / 16][16];
 #pragma unroll
-            for (int c = 0; c < NK / 32; ++c) tmem_ld32(s_at + 32 * c, s[c]);
+            for (int c = 0; c < NK / 16; ++c) tmem_ld16_async(s_at + 16 * c, s[c]);
             tmem_ld_wait();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_r + 8 * t);
             if (p.scale_log2 < 0.f)
 #pragma unroll
-                for (int c = 0; c < NK / 32; ++c)
+                for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c][i] ^= 0x80000000u;
+                    for (int i = 0; i < 16; ++i) s[c][i] ^= 0x80000000u;
             const uint32_t v0 = j * NK;
-            const bool cut = v0 + NK > hi || (lo > v0 && v0 + NK > p.sinks && lo > p.sinks);
-            if (__any_sync(0xFFFFFFFFu, cut)) {
+            if (__any_sync(0xFFFFFFFFu, v0 + NK > hi)) {
+                const uint32_t end = hi > v0 ? hi - v0 : 0;
 #pragma unroll
-                for (int c = 0; c < NK / 32; ++c)
+                for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const uint32_t v = v0 + 32 * c + i;
-                        if (v >= hi || (v >= p.sinks && v < lo)) s[c][i] = 0xFF800000u;
+                    for (int i = 0; i < 16; ++i)
+                        if (16 * c + i >= end) s[c][i] = 0xFF800000u;
+            }
+            if (__any_sync(0xFFFFFFFFu, lo > v0 && v0 + NK > p.sinks && lo > p.sinks)) {
+#pragma unroll
+                for (int c = 0; c < NK / 16; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t v = v0 + 16 * c + i;
+                        if (v >= p.sinks && v < lo) s[c][i] = 0xFF800000u;
                     }
             }
             float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < NK / 32; ++c)
+            for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
-                for (int i = 0; i < 32; i += 2)
-                    top4[(i >> 1) & 3] = fmaxf(fmaxf(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), top4[(i >> 1) & 3]);
-            const float mx = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
-            const bool raise = mx > m + PR_SLACK;
+                for (int i = 0; i < 16; i += 2) top4[(i >> 1) & 3] = max3_nan(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]), top4[(i >> 1) & 3]);
+            float mx = max3_nan(top4[0], top4[1], max3_nan(top4[2], top4[3], top4[3])) * scale;
+            // a score that is no number, or plus infinity, makes the row's sums no numbers from here on
+            if (mx == INFINITY) mx = NAN;
+            const bool raise = !(mx <= m + PR_SLACK);
             if (__any_sync(0xFFFFFFFFu, raise)) {
-                const float top = raise ? mx : m, alpha = raise ? exp2_approx(m - mx) : 1.f;
+                const float top = raise ? mx : m, alpha = raise ? exp2_approx(m - mx) : 1.f;  // 0 at first
                 m = top;
                 l *= alpha;
                 if (j) {
@@ -523,21 +619,33 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 }
             }
             const float base = m == -INFINITY ? 0.f : m - PR_BIAS<F16>;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const f32x2 scale2 = f2(scale, scale), base2 = f2(-base, -base);
+            f32x2 sum[2] = {0, 0};
+            uint32_t w8[NK / 16][8];
 #pragma unroll
-            for (int c = 0; c < NK / 32; ++c) {
-                uint32_t w16[16];
+            for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float a = exp2_approx(fmaf(__uint_as_float(s[c][2 * i]), scale, -base));
-                    const float b = exp2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), scale, -base));
-                    sum[(2 * i) & 3] += a;
-                    sum[(2 * i + 1) & 3] += b;
-                    w16[i] = pack2<F16>(a, b);
+                for (int i = 0; i < 8; ++i) {
+                    const f32x2 x = f2_fma(f2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, base2);
+                    float2 e;
+                    if ((i * PR_POLY) / 8 != ((i + 1) * PR_POLY) / 8) {
+                        e = exp2_poly(x);
+                    } else {
+                        const float2 y = f2_split(x);
+                        e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                    }
+                    sum[i & 1] = f2_add(sum[i & 1], f2(e.x, e.y));
+                    w8[c][i] = pack2<F16>(e.x, e.y);
                 }
-                tmem_st16_async(p_at + 16 * c, w16);
+            const float2 all = f2_split(f2_add(sum[0], sum[1]));
+            l += all.x + all.y;
+            if (j && !pr_wait_warp(bar_o + 8 * t, (j - 1) & 1, dead)) {  // the products that read the weights before
+                ok = false;
+                break;
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_after();
+#pragma unroll
+            for (int c = 0; c < NK / 16; ++c) tmem_st8_async(p_at + 8 * c, w8[c]);
             tmem_st_wait();
             tc_before();
             __syncwarp();
@@ -650,11 +758,11 @@ cudaError_t prompt_go(const AttnParams& p, PromptPlan& d, uint32_t grid, cudaStr
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(prompt_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<DP>::SMEM); });
     if (e != cudaSuccess) return e;
-    // the largest power of two that divides a page, if that is a whole swizzle pattern (8 rows)
+    // the largest power of two that divides a page and a tile, if that is a whole swizzle pattern (8 rows)
     CUtensorMap q = {}, k = {}, v = {};
     if (!query_map(&q, p, d)) return cudaErrorInvalidValue;
     d.rows = p.page.d & (0u - p.page.d);
-    if (d.rows > (uint32_t)PromptShape<DP>::NK) d.rows = PromptShape<DP>::NK;
+    while (PromptShape<DP>::NK % d.rows) d.rows /= 2;
     if (d.rows < 8 || !cache_map(&k, p.k, F16, p, p.k_page, p.k_tok, p.k_head, d.rows) || !cache_map(&v, p.v, F16, p, p.v_page, p.v_tok, p.v_head, d.rows))
         d.rows = 0;
     note_launch();
@@ -668,7 +776,7 @@ cudaError_t launch_prompt(const AttnParams& p, cudaStream_t st) {
     d.heads = p.group < 128 ? p.group : 128;
     d.chunks = (p.group + d.heads - 1) / d.heads;
     d.tokens = 128 / d.heads;
-    const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, nk = dp == 256 ? 64 : 128, nq = dp == 256 ? 1 : 2;
+    const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, nk = dp == 256 ? PromptShape<256>::NK : dp == 128 ? PromptShape<128>::NK : PromptShape<64>::NK, nq = dp == 256 ? 1 : 2;
     d.ksteps = (p.dim + 15) / 16;
     const uint32_t type = p.f16 ? 0u : 1u, common = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);  // f32 sums, M = 128
     d.idesc_s = common | ((nk >> 3) << 17);
