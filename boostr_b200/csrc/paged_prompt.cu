@@ -52,11 +52,11 @@ constexpr int PR_LOADERS = 128;
 template <int DP>
 struct PromptShape {
     static constexpr int NQ = DP == 256 ? 1 : 2;                        // query tiles of a CTA
-    static constexpr int NK = DP == 256 ? 64 : DP == 128 ? 80 : 128;    // keys of a tile
-    static constexpr int SLOTS = DP == 64 ? 8 : DP == 128 ? 7 : 4;      // tiles of keys or values in the ring
+    static constexpr int NK = DP == 256 ? 48 : DP == 128 ? 80 : 128;    // keys of a tile
+    static constexpr int DEPTH = DP == 64 ? 4 : 3;                      // tiles of keys, and of values, in the rings
     static constexpr int Q_TILE = 128 * DP * 2, KV_TILE = NK * DP * 2;
-    static constexpr int OFF_Q = 0, OFF_KV = NQ * Q_TILE, OFF_ROWS = OFF_KV + SLOTS * KV_TILE, OFF_BAR = OFF_ROWS + 3 * 2 * 128 * 8,
-                         SMEM = OFF_BAR + 512 + 1024;  // 1 KB of slack for the alignment of the swizzled tiles
+    static constexpr int OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + DEPTH * KV_TILE, OFF_ROWS = OFF_V + DEPTH * KV_TILE,
+                         OFF_BAR = OFF_ROWS + 3 * 2 * 128 * 8, SMEM = OFF_BAR + 512 + 1024;  // 1 KB of slack for the alignment of the swizzled tiles
     static_assert(KV_TILE % 1024 == 0 && SMEM <= 227 * 1024, "tiles of whole swizzle patterns that fit");
     // tensor memory: scores, weights, sums
     __host__ __device__ static constexpr int s_col(int t) { return t * NK; }
@@ -64,10 +64,6 @@ struct PromptShape {
     __host__ __device__ static constexpr int o_col(int t) { return 512 - (NQ - t) * DP; }
     static_assert(NQ * (NK + NK / 2 + DP) <= 512, "tensor memory");
 };
-// Items of the ring: K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1), as the products take them.
-__device__ __forceinline__ uint32_t item_k(uint32_t j) { return j ? 2 * j - 1 : 0; }
-__device__ __forceinline__ uint32_t item_v(uint32_t j, uint32_t n) { return j + 1 == n ? 2 * n - 1 : 2 * j + 2; }
-
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
@@ -237,14 +233,16 @@ template <int DP, bool F16>
 __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams p, const PromptPlan d, const __grid_constant__ CUtensorMap map_q,
                                                                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using Sh = PromptShape<DP>;
-    constexpr int NQ = Sh::NQ, NK = Sh::NK, SLOTS = Sh::SLOTS;
+    constexpr int NQ = Sh::NQ, NK = Sh::NK, DEPTH = Sh::DEPTH;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
     const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t bar = sbase + Sh::OFF_BAR;
-    // queries there; of a query tile: scores computed, scores read, weights written, values added; of a slot: filled, free
-    const uint32_t bar_q = bar, bar_s = bar + 8, bar_r = bar + 24, bar_p = bar + 40, bar_o = bar + 56, bar_full = bar + 80, bar_empty = bar + 80 + 8 * SLOTS;
+    // queries there; of a query tile: scores computed, scores read (and the weights before them written), last weights written, values
+    // added; of a slot: keys there, values there; step done (slot j % DEPTH: values j and keys j + 2 have been used)
+    const uint32_t bar_q = bar, bar_s = bar + 8, bar_r = bar + 24, bar_p = bar + 40, bar_o = bar + 56, bar_k = bar + 72, bar_v = bar_k + 8 * DEPTH,
+                   bar_done = bar_v + 8 * DEPTH;
     volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 256);
     volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 260);
     __shared__ uint32_t s_scan[PR_THREADS / 32], s_find[2];
@@ -303,10 +301,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 mbar_init(bar_p + 8 * t, 4);
                 mbar_init(bar_o + 8 * t, 1);
             }
-            for (int i = 0; i < SLOTS; ++i) {
-                mbar_init(bar_full + 8 * i, 1);
-                mbar_init(bar_empty + 8 * i, 1);
-            }
+            for (int i = 0; i < 3 * DEPTH; ++i) mbar_init(bar_k + 8 * i, i < 2 * DEPTH ? 1 : NQ);
             *dead = 0;
             mbar_fence_init();
         }
@@ -341,22 +336,23 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12 && nt && elect_one_lane()) {
+        const uint32_t t = warp - 12;
+        if (t < NQ && nt && elect_one_lane()) {
             // -------------------------------------------------------------------------------------------- MMA issue
-            // One thread: what it does between two products is time in which the tensor core may run dry.  Descriptors by their low
-            // words, so that what changes from one product to the next is a sum.
-            const uint32_t q_lo = desc_lo(sbase + Sh::OFF_Q), k_lo = desc_lo(sbase + Sh::OFF_KV);
-            const uint32_t v_lo = (((sbase + Sh::OFF_KV) >> 4) & 0x3FFFu) | (uint32_t)((NK * 128) >> 4) << 16;
+            // A thread for each query tile: the waits of one overlap the products of the other.  (One thread for both: 594 us in place of
+            // 562 for 8192 tokens.)  Descriptors by their low words, so that what changes from one product to the next is a sum.
+            const uint32_t q_lo = desc_lo(sbase + Sh::OFF_Q), k_lo = desc_lo(sbase + Sh::OFF_K);
+            const uint32_t v_lo = (((sbase + Sh::OFF_V) >> 4) & 0x3FFFu) | (uint32_t)((NK * 128) >> 4) << 16;
             bool ok = true;
             auto wait = [&](uint32_t b, uint32_t phase) {
                 if (ok && !pr_wait(b, phase & 1, dead)) ok = false;
                 tc_after();
             };
-            auto scores = [&](uint32_t t, uint32_t slot) {
+            auto scores = [&](uint32_t slot) {
                 if (!ok) return;
-                const uint32_t q = q_lo + t * (Sh::Q_TILE >> 4), k = k_lo + slot * (Sh::KV_TILE >> 4);
+                const uint32_t q = q_lo + t * (Sh::Q_TILE >> 4), k = k_lo + slot * (Sh::KV_TILE >> 4), to = tmem + t * NK;
                 auto product = [&](uint32_t i) {
-                    tc_mma_ss(tmem + Sh::s_col(t), desc_sw128(q + (i >> 2) * ((128 * 128) >> 4) + (i & 3) * 2),
+                    tc_mma_ss(to, desc_sw128(q + (i >> 2) * ((128 * 128) >> 4) + (i & 3) * 2),
                               desc_sw128(k + (i >> 2) * ((NK * 128) >> 4) + (i & 3) * 2), d.idesc_s, i != 0);
                 };
                 if (d.ksteps == DP / 16) {
@@ -370,61 +366,42 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             };
             // The values as they lie: rows of 64 elements are the K dimension ("MN-major"), 8-row groups 1024 bytes apart (the descriptor's
             // stride), blocks of 64 elements NK * 128 bytes apart (its leading dimension)
-            auto values = [&](uint32_t t, uint32_t slot, bool accumulate) {
+            auto values = [&](uint32_t slot, bool accumulate) {
                 if (!ok) return;
-                const uint32_t v = v_lo + slot * (Sh::KV_TILE >> 4);
+                const uint32_t v = v_lo + slot * (Sh::KV_TILE >> 4), to = tmem + Sh::o_col(0) + t * DP, from = tmem + Sh::p_col(0) + t * (NK / 2);
 #pragma unroll
-                for (uint32_t i = 0; i < NK / 16; ++i)
-                    tc_mma_ts(tmem + Sh::o_col(t), tmem + Sh::p_col(t) + 8 * i, desc_sw128(v + i * (2048 >> 4)), d.idesc_o, accumulate || i);
+                for (uint32_t i = 0; i < NK / 16; ++i) tc_mma_ts(to, from + 8 * i, desc_sw128(v + i * (2048 >> 4)), d.idesc_o, accumulate || i);
                 tc_commit_to(bar_o + 8 * t);
             };
-            // the items of the ring in their order: the current one's slot and phase
-            uint32_t slot = 0, phase = 0;
-            auto advance = [&]() {
-                if (ok) tc_commit_to(bar_empty + 8 * slot);  // free when the products so far are done
-                if (++slot == SLOTS) slot = 0, phase ^= 1;
-            };
-            wait(bar_q, 0);
-            // While a tile's weights are computed, its next scores are, too; the products of the two tiles alternate.
-            wait(bar_full, 0);
-#pragma unroll
-            for (uint32_t t = 0; t < NQ; ++t)
-                if (t < nq && (t == nq - 1 ? nt : n0) > 0) scores(t, 0);
-            advance();
-            if (nt > 1) {
-                wait(bar_full + 8 * slot, phase);
-#pragma unroll
-                for (uint32_t t = 0; t < NQ; ++t)
-                    if (t < nq && (t == nq - 1 ? nt : n0) > 1) {
-                        wait(bar_r + 8 * t, 0);
-                        scores(t, slot);
-                    }
-                advance();
+            const uint32_t mine = t >= nq ? 0 : t == nq - 1 ? nt : n0;
+            if (mine) wait(bar_q, 0);
+            for (uint32_t j = 0; j < 2 && j < mine; ++j) {
+                wait(bar_k + 8 * j, 0);
+                if (j) wait(bar_r + 8 * t, 0);
+                scores(j);
             }
+            // Step j: the values of tile j and the scores of tile j + 2.  The scores of tile j + 1 have been computed before, and that they
+            // have been read says that the weights of tile j are written; so the softmax waits for nothing while products run.
+            uint32_t vs = 0, vp = 0, ks = 2 % DEPTH, kp = 2 / DEPTH;  // slots and phases of values j and keys j + 2
             for (uint32_t j = 0; ok && j < nt; ++j) {
-                // values of tile j in this slot, keys of tile j + 2 in the next
-                const uint32_t next = slot + 1 == SLOTS ? 0 : slot + 1, next_phase = slot + 1 == SLOTS ? phase ^ 1 : phase;
-                bool have_v = false, have_k = false;
-#pragma unroll
-                for (uint32_t t = 0; t < NQ; ++t) {
-                    const uint32_t mine = t == nq - 1 ? nt : n0;
-                    if (t >= nq || j >= mine) continue;
-                    if (!have_v) wait(bar_full + 8 * slot, phase);
-                    have_v = true;
-                    wait(bar_p + 8 * t, j);
-                    values(t, slot, j != 0);
+                wait(bar_v + 8 * vs, vp);
+                if (j < mine) {
+                    if (j + 1 < mine) wait(bar_r + 8 * t, j + 1);
+                    else wait(bar_p + 8 * t, 0);
+                    values(vs, j != 0);
                     if (j + 2 < mine) {
-                        if (!have_k) wait(bar_full + 8 * next, next_phase);
-                        have_k = true;
-                        wait(bar_r + 8 * t, j + 1);
-                        scores(t, next);
+                        wait(bar_k + 8 * ks, kp);
+                        scores(ks);
                     }
+                    if (ok) tc_commit_to(bar_done + 8 * vs);
+                } else if (ok) {
+                    mbar_arrive(bar_done + 8 * vs);  // a tile that is done uses nothing
                 }
-                advance();
-                if (j + 2 < nt) advance();
+                if (++vs == DEPTH) vs = 0, vp ^= 1;
+                if (++ks == DEPTH) ks = 0, kp ^= 1;
             }
             // the last commit has arrived before the block ends (those before it then have, too)
-            if (ok) ok = pr_wait(bar_empty + 8 * ((2 * nt - 1) % SLOTS), ((2 * nt - 1) / SLOTS) & 1, dead);
+            if (ok) ok = pr_wait(bar_done + 8 * ((nt - 1) % DEPTH), ((nt - 1) / DEPTH) & 1, dead);
             if (!ok) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
         }
         __syncwarp();
@@ -458,47 +435,49 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                                     w.row0 + t * d.tokens, bar_q);
             }
             __syncwarp();
-            // Whole tiles come by TMA where boxes fit into pages: the warps take the items in turn, a lane finds the pages of a box, one
-            // lane issues them all.
-            const uint32_t whole = d.rows ? w.keys / NK : 0, lw = tid >> 5;  // tiles by TMA
-            if (whole) {
-                const uint32_t groups = NK / d.rows, last = whole == nt ? 2 * nt : 2 * nt - 1;
-                uint32_t slot = lw, par = 1;  // par: of the slot's last release; the first round waits for nothing
-                for (uint32_t item = lw; ok && item < last; item += 4) {
-                    const uint32_t kv = item + 1 == 2 * nt || (item && !(item & 1)), j = item + 1 == 2 * nt ? nt - 1 : kv ? item / 2 - 1 : (item + 1) / 2;
-                    if (j < whole) {
-                        uint32_t page = 0, tok = 0;
-                        if (lane < groups) {
-                            const uint32_t v = j * NK + lane * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
-                            if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
-                        }
-                        if (item >= SLOTS) ok = pr_wait_warp(bar_empty + 8 * slot, par, dead);
-                        const uint32_t dst = sbase + Sh::OFF_KV + slot * Sh::KV_TILE, full = bar_full + 8 * slot;
-                        if (ok && lane == 0) mbar_expect_tx(full, groups * blocks * d.rows * 128);
-                        for (uint32_t g = 0; g < groups; ++g) {
-                            const uint32_t pg = __shfl_sync(0xFFFFFFFFu, page, g), tk = __shfl_sync(0xFFFFFFFFu, tok, g);
-                            if (ok && lane == 0)
-                                for (uint32_t b = 0; b < blocks; ++b)
-                                    tma_rows(dst + b * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * b, w.head, tk, pg, full);
-                        }
-                        __syncwarp();
-                    }
-                    slot += 4;
-                    if (slot >= SLOTS) slot -= SLOTS, par ^= 1;
+            // Keys i take the place of keys i - DEPTH, which are used up with step i - DEPTH - 2 (the first two before step 0); values i that
+            // of values i - DEPTH, used in the step of that number.
+            auto room = [&](uint32_t kv, uint32_t i) {
+                if (!ok || i < DEPTH) return;
+                const uint32_t step = kv ? i - DEPTH : i >= DEPTH + 2 ? i - DEPTH - 2 : 0;
+                ok = pr_wait_warp(bar_done + 8 * (step % DEPTH), (step / DEPTH) & 1, dead);
+            };
+            // Whole tiles come by TMA where boxes fit into pages.  Two warps take the keys in turn, two the values; a lane finds the pages of a
+            // box, one lane issues them all.
+            const uint32_t whole = d.rows ? w.keys / NK : 0, kv = (tid >> 5) & 1;  // tiles by TMA
+            for (uint32_t i = tid >> 6; ok && i < whole; i += 2) {
+                const uint32_t groups = NK / d.rows, slot = i % DEPTH;
+                uint32_t page = 0, tok = 0;
+                if (lane < groups) {
+                    const uint32_t v = i * NK + lane * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
+                    if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
                 }
+                room(kv, i);
+                const uint32_t dst = sbase + (kv ? Sh::OFF_V : Sh::OFF_K) + slot * Sh::KV_TILE, full = (kv ? bar_v : bar_k) + 8 * slot;
+                if (ok && lane == 0) mbar_expect_tx(full, groups * blocks * d.rows * 128);
+                for (uint32_t g = 0; g < groups; ++g) {
+                    const uint32_t pg = __shfl_sync(0xFFFFFFFFu, page, g), tk = __shfl_sync(0xFFFFFFFFu, tok, g);
+                    if (ok && lane == 0)
+                        for (uint32_t b = 0; b < blocks; ++b)
+                            tma_rows(dst + b * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * b, w.head, tk, pg, full);
+                }
+                __syncwarp();
             }
-            // Other caches, and the last tile: by copies that fill the rows behind the last visible key with zeros.  An item is announced
-            // when LAG younger ones are on their way.  (A slot is free when the item in it and the one behind that have been used, and
-            // those were announced long before the slot comes round: SLOTS > LAG + 1.)
-            constexpr uint32_t LAG = 2;
+            // Other caches, and the last tile: by copies that fill the rows behind the last visible key with zeros, in the order in which the
+            // products need them (K0 K1 V0 K2 V1 ...).  A copy is announced when one younger is on its way: the step that the younger
+            // one's room waits for needs none behind the one announced (keys i: step i - DEPTH - 2 needs keys i - DEPTH, keys DEPTH: step
+            // 0 needs keys 2; values i: step i - DEPTH needs keys i - DEPTH + 2).
+            constexpr uint32_t LAG = 1;
             uint32_t copied = 0, told = 0;
             auto announce = [&](uint32_t upto) {  // the caller has waited for its own copies
                 proxy_fence();
                 named_bar_sync(1, PR_LOADERS);
                 if (tid == 0)
                     for (uint32_t i = told; i < upto; ++i) {
-                        const uint32_t item = !whole ? i : i ? 2 * nt - 1 : item_k(nt - 1);
-                        mbar_arrive(bar_full + 8 * (item % SLOTS));
+                        // copy i is that of keys 0, keys 1, values 0, keys 2, ... (from tile `whole` on), then the last values
+                        const bool is_v = i + 1 == 2 * (nt - whole) || (i && !(i & 1));
+                        const uint32_t of = whole + (i + 1 == 2 * (nt - whole) ? nt - whole - 1 : is_v ? i / 2 - 1 : (i + 1) / 2);
+                        mbar_arrive((is_v ? bar_v : bar_k) + 8 * (of % DEPTH));
                     }
                 told = upto;
             };
@@ -520,10 +499,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 // keys of tile j, then values of the tile before (and, behind the last keys, of the last one)
                 for (uint32_t k = 0; k < 3; ++k) {
                     if ((k == 1 && j == whole) || (k == 2 && j + 1 < nt)) continue;
-                    const uint32_t of = k == 1 ? j - 1 : j, item = k ? item_v(of, nt) : item_k(of), slot = item % SLOTS;
-                    if (ok && item >= SLOTS) ok = pr_wait_warp(bar_empty + 8 * slot, (item / SLOTS - 1) & 1, dead);
+                    const uint32_t of = k == 1 ? j - 1 : j;
+                    room(k, of);
                     // a CTA that gave up: the copies still end, into slots that nobody reads
-                    copy(sbase + Sh::OFF_KV + slot * Sh::KV_TILE, rows + of % 3 * 256 + (k ? 128 : 0), NK);
+                    copy(sbase + (k ? Sh::OFF_V : Sh::OFF_K) + of % DEPTH * Sh::KV_TILE, rows + of % 3 * 256 + (k ? 128 : 0), NK);
                     if (++copied > told + LAG) {
                         cp_async_wait<LAG>();
                         announce(copied - LAG);
@@ -558,6 +537,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 break;
             }
             tc_after();
+            auto values_done = [&]() {  // the values of tile j - 1 are added
+                const bool r = pr_wait_warp(bar_o + 8 * t, (j - 1) & 1, dead);
+                tc_after();
+                return r;
+            };
             uint32_t s[NK / 16][16];
 #pragma unroll
             for (int c = 0; c < NK / 16; ++c) tmem_ld16_async(s_at + 16 * c, s[c]);
@@ -602,11 +586,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 m = top;
                 l *= alpha;
                 if (j) {
-                    if (!pr_wait_warp(bar_o + 8 * t, (j - 1) & 1, dead)) {
+                    if (!values_done()) {
                         ok = false;
                         break;
                     }
-                    tc_after();
 #pragma unroll 1
                     for (uint32_t c = 0; c < p.dim; c += 16) {
                         uint32_t o[16];
@@ -639,17 +622,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 }
             const float2 all = f2_split(f2_add(sum[0], sum[1]));
             l += all.x + all.y;
-            if (j && !pr_wait_warp(bar_o + 8 * t, (j - 1) & 1, dead)) {  // the products that read the weights before
+            if (j && !values_done()) {  // they read the weights before these
                 ok = false;
                 break;
             }
-            tc_after();
 #pragma unroll
             for (int c = 0; c < NK / 16; ++c) tmem_st8_async(p_at + 8 * c, w8[c]);
             tmem_st_wait();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p + 8 * t);
+            if (j + 1 == mine) {  // otherwise the next scores' reading says so
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_p + 8 * t);
+            }
         }
         if (!ok && lane == 0) pr_fail(dead, p.status, STATUS_TIMEOUT_MMA);
         // ---- the rows' sums
