@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 mbar_init(bar_p + 8 * t, 4);
                 mbar_init(bar_o + 8 * t, 1);
             }
-            for (int i = 0; i < 3 * DEPTH; ++i) mbar_init(bar_k + 8 * i, i < 2 * DEPTH ? 1 : NQ);
+            for (int i = 0; i < 3 * DEPTH; ++i) mbar_init(bar_k + 8 * i, i < 2 * DEPTH ? 4 : NQ);
             *dead = 0;
             mbar_fence_init();
         }
@@ -442,26 +442,29 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 const uint32_t step = kv ? i - DEPTH : i >= DEPTH + 2 ? i - DEPTH - 2 : 0;
                 ok = pr_wait_warp(bar_done + 8 * (step % DEPTH), (step / DEPTH) & 1, dead);
             };
-            // Whole tiles come by TMA where boxes fit into pages.  Two warps take the keys in turn, two the values; a lane finds the pages of a
-            // box, one lane issues them all.
-            const uint32_t whole = d.rows ? w.keys / NK : 0, kv = (tid >> 5) & 1;  // tiles by TMA
-            for (uint32_t i = tid >> 6; ok && i < whole; i += 2) {
-                const uint32_t groups = NK / d.rows, slot = i % DEPTH;
-                uint32_t page = 0, tok = 0;
-                if (lane < groups) {
-                    const uint32_t v = i * NK + lane * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
-                    if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
+            // Whole tiles come by TMA where boxes fit into pages: a lane finds the page of a box and issues it.  A warp takes 200 cycles for each
+            // box, so all four share every tile (one warp a tile: the keys came late).
+            const uint32_t whole = d.rows ? w.keys / NK : 0, lw = tid >> 5;  // tiles by TMA
+            if (whole) {
+                const uint32_t boxes = NK / d.rows * blocks, own = (boxes + 3 - lw) / 4, box = lw + 4 * lane, g = box / blocks, b = box - g * blocks;
+                auto tile = [&](uint32_t kv, uint32_t i) {
+                    uint32_t page = 0, tok = 0;
+                    if (lane < own) {
+                        const uint32_t v = i * NK + g * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
+                        if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
+                    }
+                    room(kv, i);
+                    if (!ok) return;
+                    const uint32_t dst = sbase + (kv ? Sh::OFF_V : Sh::OFF_K) + i % DEPTH * Sh::KV_TILE, full = (kv ? bar_v : bar_k) + 8 * (i % DEPTH);
+                    if (lane == 0) mbar_expect_tx(full, own * d.rows * 128);
+                    __syncwarp();
+                    if (lane < own) tma_rows(dst + b * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * b, w.head, tok, page, full);
+                    __syncwarp();
+                };
+                for (uint32_t i = 0; i <= whole; ++i) {  // K0 K1 V0 K2 V1 ...
+                    if (i < whole) tile(0, i);
+                    if (i) tile(1, i - 1);
                 }
-                room(kv, i);
-                const uint32_t dst = sbase + (kv ? Sh::OFF_V : Sh::OFF_K) + slot * Sh::KV_TILE, full = (kv ? bar_v : bar_k) + 8 * slot;
-                if (ok && lane == 0) mbar_expect_tx(full, groups * blocks * d.rows * 128);
-                for (uint32_t g = 0; g < groups; ++g) {
-                    const uint32_t pg = __shfl_sync(0xFFFFFFFFu, page, g), tk = __shfl_sync(0xFFFFFFFFu, tok, g);
-                    if (ok && lane == 0)
-                        for (uint32_t b = 0; b < blocks; ++b)
-                            tma_rows(dst + b * (NK * 128) + g * d.rows * 128, kv ? &map_v : &map_k, 64 * b, w.head, tk, pg, full);
-                }
-                __syncwarp();
             }
             // Other caches, and the last tile: by copies that fill the rows behind the last visible key with zeros, in the order in which the
             // products need them (K0 K1 V0 K2 V1 ...).  A copy is announced when one younger is on its way: the step that the younger
@@ -471,8 +474,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             uint32_t copied = 0, told = 0;
             auto announce = [&](uint32_t upto) {  // the caller has waited for its own copies
                 proxy_fence();
-                named_bar_sync(1, PR_LOADERS);
-                if (tid == 0)
+                __syncwarp();
+                if (lane == 0)
                     for (uint32_t i = told; i < upto; ++i) {
                         // copy i is that of keys 0, keys 1, values 0, keys 2, ... (from tile `whole` on), then the last values
                         const bool is_v = i + 1 == 2 * (nt - whole) || (i && !(i & 1));
@@ -528,6 +531,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         const uint32_t mine = t >= nq ? 0 : t == nq - 1 ? nt : n0;
         const uint32_t lanes = tmem + (((uint32_t)(warp & 3) * 32u) << 16);
         const uint32_t s_at = lanes + Sh::s_col(t), p_at = lanes + Sh::p_col(t), o_at = lanes + Sh::o_col(t);
+        // tiles in which a row of the warp has limits: from open_end on, and in [cut_from, cut_to)
+        const uint32_t open_end = __reduce_min_sync(0xFFFFFFFFu, hi) / NK, cut_from = p.sinks / NK;
+        const uint32_t cut_to = (__reduce_max_sync(0xFFFFFFFFu, lo > p.sinks ? lo : 0u) + NK - 1) / NK;
         const float scale = fabsf(p.scale_log2);
         float m = -INFINITY, l = 0.f;  // m: of the scaled scores
         bool ok = true;
@@ -554,23 +560,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[c][i] ^= 0x80000000u;
-            const uint32_t v0 = j * NK;
-            if (__any_sync(0xFFFFFFFFu, v0 + NK > hi)) {
-                const uint32_t end = hi > v0 ? hi - v0 : 0;
+            if (j >= open_end) {
+                const int end = (int)min(hi, 0x40000000u) - (int)(j * NK);
 #pragma unroll
                 for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (16 * c + i >= end) s[c][i] = 0xFF800000u;
             }
-            if (__any_sync(0xFFFFFFFFu, lo > v0 && v0 + NK > p.sinks && lo > p.sinks)) {
+            if (j >= cut_from && j < cut_to) {  // [a, a + n) is hidden
+                const int a = (int)p.sinks - (int)(j * NK);
+                const uint32_t n = lo > p.sinks ? lo - p.sinks : 0;
 #pragma unroll
                 for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint32_t v = v0 + 16 * c + i;
-                        if (v >= p.sinks && v < lo) s[c][i] = 0xFF800000u;
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        if ((uint32_t)(16 * c + i - a) < n) s[c][i] = 0xFF800000u;
             }
             float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
