@@ -9,7 +9,7 @@ namespace b200q {
 size_t slots_max_requests();
 cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st);
 cudaError_t launch_rope(const RopeParams& p, int dtype, bool interleaved, uint32_t run, cudaStream_t st);
-cudaError_t launch_prompt(const AttnParams& p, cudaStream_t st);
+cudaError_t launch_prompt(const AttnParams& p, int sm_count, cudaStream_t st);
 size_t decode_workspace_bytes(uint32_t group, uint32_t dim, int sm_count);
 cudaError_t launch_decode(const AttnParams& p, void* ws, int sm_count, cudaStream_t st);
 }  // namespace b200q
@@ -175,7 +175,7 @@ int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t
                            scale, window, sinks, out, out_dtype, lse))
         return rc;
     p.cu = cu_seqlens;
-    return finish(op, launch_prompt(p, static_cast<cudaStream_t>(stream)));
+    return finish(op, launch_prompt(p, api_sm_count(), static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"
