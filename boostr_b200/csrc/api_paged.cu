@@ -121,7 +121,7 @@ int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, const b200q_he
     p.tokens = (uint32_t)tokens, p.hq = (uint32_t)q_heads, p.hkv = (uint32_t)cache->kv_heads, p.dim = (uint32_t)cache->head_dim, p.rot = (uint32_t)rot;
     p.heads.set(p.hq + 2 * p.hkv);
     p.positions = positions, p.cos = cos, p.sin = sin, p.table_rows = rot ? (uint32_t)table_rows : 0xFFFFFFFFu;
-    p.q_weight = q_weight, p.k_weight = k_weight, p.eps = eps;
+    p.q_weight = q_weight, p.k_weight = k_weight, p.eps = eps, p.inv_dim = 1.f / (float)p.dim;
     p.slots = slots, p.out = out, p.out_dtype = out_dtype;
     p.k_cache = static_cast<uint8_t*>(cache->k), p.v_cache = static_cast<uint8_t*>(cache->v);
     p.kc_page = cache->k_strides[0], p.kc_tok = cache->k_strides[1], p.kc_head = cache->k_strides[2];
@@ -136,7 +136,8 @@ int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, const b200q_he
         const int64_t r = run;
         const size_t bi = in * run < 16 ? in * run : 16, bo = type_bytes(out_dtype) * run < 16 ? type_bytes(out_dtype) * run : 16;
         if ((rot / 2) % run == 0 && p.q_row % r == 0 && p.q_head % r == 0 && p.k_row % r == 0 && p.k_head % r == 0 && p.v_row % r == 0 &&
-            p.v_head % r == 0 && aligned(p.q, bi) && aligned(p.k, bi) && aligned(p.v, bi) && aligned(p.out, bo))
+            p.v_head % r == 0 && aligned(p.q, bi) && aligned(p.k, bi) && aligned(p.v, bi) && aligned(p.out, bo) &&
+            aligned(cos, 16) && aligned(sin, 16) && aligned(q_weight, 16) && aligned(k_weight, 16))
             break;
     }
     return finish(op, launch_rope(p, dtype, interleaved != 0, run, static_cast<cudaStream_t>(stream)));

@@ -108,6 +108,14 @@ at::Tensor empty(c10::IntArrayRef shape, at::ScalarType t, c10::Device dev) {
     return at::Tensor(at::detail::empty_cuda(shape, t, dev, std::nullopt));
 }
 
+// [n] elements of type t at `byte` of another tensor's storage (a view, without a walk through the dispatcher).
+at::Tensor part_of(const at::Tensor& of, at::ScalarType t, int64_t byte, int64_t n) {
+    at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(of.storage()), of.key_set(), c10::scalarTypeToTypeMeta(t));
+    r.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    r.unsafeGetTensorImpl()->set_storage_offset(byte / (int64_t)c10::elementSize(t));
+    return r;
+}
+
 int dtype_code(at::ScalarType t) {
     switch (t) {
     case at::kFloat: return B200Q_F32;
@@ -494,8 +502,14 @@ PyObject* paged_slots(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             !size_of(args[3], page) || !page || !size_of(args[6], tokens))
             return not_served();
         DeviceScope dev(d);
-        const at::Tensor out[5] = {empty({n}, at::kInt, d), empty({n + 1}, at::kInt, d), empty({(int64_t)tokens}, at::kInt, d),
-                                   empty({(int64_t)tokens}, at::kLong, d), empty({2}, at::kInt, d)};
+        // one allocation for the five results: slots, then the 32-bit ones
+        const int64_t len[5] = {n, n + 1, (int64_t)tokens, (int64_t)tokens, 2};
+        int64_t at[5], bytes = ((int64_t)tokens * 8 + 15) / 16 * 16;
+        for (int i : {0, 1, 2, 4}) at[i] = bytes, bytes += (len[i] * 4 + 15) / 16 * 16;
+        at[3] = 0;
+        const at::Tensor all = empty({(bytes + 16) / 8}, at::kLong, d);
+        at::Tensor out[5];
+        for (int i = 0; i < 5; ++i) out[i] = part_of(all, i == 3 ? at::kLong : at::kInt, at[i], len[i]);
         const int rc = with_scratch(d, 0, [&](void*, size_t, cudaStream_t st) {
             return b200q_paged_slots(ctx->data_ptr<int>(), fresh->data_ptr<int>(), (size_t)n, table->data_ptr<int>(), table->stride(0), (size_t)table->size(1),
                                      page, free->data_ptr<int>(), (size_t)free->numel(), count->data_ptr<int>(), out[0].data_ptr<int>(),

@@ -68,7 +68,7 @@ struct RopeParams {
     const float *cos, *sin;            // [table_rows, rot / 2]
     uint32_t table_rows;
     const float *q_weight, *k_weight;  // [dim] or nullptr
-    float eps;
+    float eps, inv_dim;
     const int64_t* slots;
     void* out;                         // [tokens, hq, dim]
     int out_dtype;
