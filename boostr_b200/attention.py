@@ -237,6 +237,16 @@ def _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, si
 _decode_ws: dict = {}
 
 
+def decode_workspace(q_heads: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """Scratch for ``paged_decode``, zeroed.  The calls of one stream, or of one graph, may share it; a captured call that is given
+    none takes one of its own and zeroes it in every replay."""
+    with torch.cuda.device(torch.device(device)):
+        need = _cabi.lib().b200q_paged_decode_workspace_bytes(q_heads, kv_heads, head_dim)
+    if not need:
+        raise QuantError(f"paged_decode: {q_heads} query heads, {kv_heads} key-value heads and head_dim {head_dim} do not go together")
+    return torch.zeros(need, dtype=torch.uint8, device=device)
+
+
 def _decode_workspace(nbytes: int, device) -> torch.Tensor:
     """Scratch of ``paged_decode``, whose counters are zero between calls: one for each device and stream; a call that is being
     captured gets one of its own, zeroed by the graph."""
@@ -254,16 +264,17 @@ def _decode_workspace(nbytes: int, device) -> torch.Tensor:
 
 def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                  scale: Optional[float] = None, window: int = 0, sinks: int = 0, out_dtype: Optional[torch.dtype] = None,
-                 out: Optional[torch.Tensor] = None, return_lse: bool = False):
+                 out: Optional[torch.Tensor] = None, return_lse: bool = False, workspace: Optional[torch.Tensor] = None):
     """Attention of the newest token of each request over its pages (``b200q_paged_decode``).
 
     q [requests, q_heads, head_dim], F32 or of the cache's type; ``seq_lens[b]`` tokens of request b are in the cache, the newest
     among them.  ``scale`` is head_dim ** -0.5 unless given.  ``window`` > 0: the newest ``window`` tokens and the first ``sinks`` are
     visible.  A request of length 0 (a padded row) gives zeros.  Returns out [requests, q_heads, head_dim], of q's type
-    unless ``out_dtype`` says otherwise, and with ``return_lse`` also the log-sum-exp of the scores [requests, q_heads] f32."""
+    unless ``out_dtype`` says otherwise, and with ``return_lse`` also the log-sum-exp of the scores [requests, q_heads] f32.
+    ``workspace``: of ``decode_workspace``."""
     code = -1 if out_dtype is None else _DT.get(out_dtype)
     if code is not None:
-        r = hostops().paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, code, out, return_lse)
+        r = hostops().paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, window, sinks, code, out, return_lse, workspace)
         if _served(r):
             return r
     op = "paged_decode"
@@ -274,7 +285,9 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     lse = torch.empty(n, hq, dtype=torch.float32, device=q.device) if return_lse else None
     L = _cabi.lib()
     with torch.cuda.device(q.device):
-        ws = _decode_workspace(L.b200q_paged_decode_workspace_bytes(hq, k_cache.shape[2], d), q.device)
+        if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != q.device):
+            raise QuantError(f"{op}: workspace must be a contiguous torch.uint8 tensor on {q.device}")
+        ws = workspace if workspace is not None else _decode_workspace(L.b200q_paged_decode_workspace_bytes(hq, k_cache.shape[2], d), q.device)
         _cabi.check(L.b200q_paged_decode(q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), n, hq, cache, block_table.data_ptr(),
                                          block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), scale, window, sinks, out.data_ptr(),
                                          _DT[out.dtype], lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), _stream()))

@@ -462,8 +462,12 @@ at::ScalarType out_type(PyObject* given, long code, const at::Tensor& q) {
 // each (device, stream), and one of its own for a call that is being captured, zeroed by the graph.
 auto& g_counters = *new std::map<std::pair<int, cudaStream_t>, std::unique_ptr<Scratch>>;
 template <typename F>
-int with_counters(c10::Device dev, size_t need, F&& call) {
+int with_counters(c10::Device dev, size_t need, const at::Tensor* given, F&& call) {
     const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    if (given) {
+        NoGil nogil;
+        return call(given->data_ptr(), (size_t)given->numel(), st);
+    }
     if (capturing(st)) {
         const at::Tensor buf = empty({(int64_t)need}, at::kByte, dev);
         NoGil nogil;
@@ -622,16 +626,19 @@ PyObject* attn_result(int rc, const Attn& a) {
     return r;
 }
 
+// paged_decode(..., as above, workspace or None)
 PyObject* paged_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return guarded([&]() -> PyObject* {
         Attn a;
-        if (nargs != 11 || !THPVariable_CheckExact(args[0]) || !THPVariable_Unpack(args[0]).is_cuda()) return not_served();
+        if (nargs != 12 || !THPVariable_CheckExact(args[0]) || !THPVariable_Unpack(args[0]).is_cuda()) return not_served();
         const c10::Device d = THPVariable_Unpack(args[0]).device();
         DeviceScope dev(d);
         if (!attn_of(args, a) || a.lens->size(0) != a.q->size(0)) return not_served();
         const size_t need = b200q_paged_decode_workspace_bytes((size_t)a.q->size(1), a.c.kv_heads, a.c.head_dim);
         if (!need) return not_served();
-        const int rc = with_counters(d, need, [&](void* ws, size_t bytes, cudaStream_t st) {
+        const at::Tensor* given = args[11] == Py_None ? nullptr : tensor_of(args[11], at::kByte, d);
+        if (args[11] != Py_None && (!given || !given->is_contiguous())) return not_served();
+        const int rc = with_counters(d, need, given, [&](void* ws, size_t bytes, cudaStream_t st) {
             return b200q_paged_decode(a.q->data_ptr(), dtype_code(a.q->scalar_type()), a.q->stride(0), a.q->stride(1), (size_t)a.q->size(0),
                                       (size_t)a.q->size(1), &a.c, a.table->data_ptr<int>(), a.table->stride(0), (size_t)a.table->size(1),
                                       a.lens->data_ptr<int>(), a.scale, a.window, a.sinks, a.out.data_ptr(), a.odt,

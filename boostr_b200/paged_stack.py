@@ -1,0 +1,139 @@
+"""A LLaMA-shaped decoder that serves requests: quantized linears, and attention from a paged key-value cache between them.
+
+``PagedStack`` keeps the cache, the block tables and the lengths of a fixed number of requests on the GPU.  ``prompt`` takes ragged
+runs of new tokens (whole prompts, or chunks of them) through all layers, ``step`` one token of each request; ``capture`` makes
+the step a graph whose replays advance lengths and tables by themselves.  Tokens enter as hidden states and leave as logits of
+each request's newest token: embeddings and sampling belong to the host model.
+
+Per layer, as boostr's block does (src/model/llama/model/blocks_attention.rs, blocks_mlp.rs): RMSNorm + q/k/v as one operator,
+``rope_append``, ``paged_decode`` or ``paged_prompt``, output projection, RMSNorm, feed-forward block, residuals around both.
+
+``python -m boostr_b200.paged_stack`` serves a few requests of a Llama-3-8B-shaped model with random weights and prints the rates."""
+from __future__ import annotations
+
+import argparse
+import time
+from typing import Optional, Sequence
+
+import torch
+
+from . import attention, ops, synth
+from .decode_graph import DecodeGraph
+from .decode_stack import FFN, HIDDEN, KV, LAYERS, VOCAB, layer_spec
+
+
+class PagedStack:
+    def __init__(self, requests: int, pages: int, page_size: int = 16, max_pages: int = 512, layers: int = LAYERS, hidden: int = HIDDEN,
+                 kv: int = KV, ffn: int = FFN, vocab: int = VOCAB, head_dim: int = 128, rope_base: float = 500000.0,
+                 rope_scaling: Optional[dict] = None, window: int = 0, sinks: int = 0, head_norms: bool = False, eps: float = 1e-5, seed: int = 0xB200):
+        self.requests, self.page_size, self.window, self.sinks, self.eps = requests, page_size, window, sinks, eps
+        self.hidden, self.head_dim, self.q_heads, self.kv_heads = hidden, head_dim, hidden // head_dim, kv // head_dim
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(seed)
+        norm = lambda n: 1 + 0.1 * torch.randn(n, generator=gen, device="cuda")  # noqa: E731
+        self.layers = []
+        for _ in range(layers):
+            L = {name: synth.device_weight(fmt, n, k, gen) for name, fmt, n, k, _ in layer_spec(hidden, kv, ffn)}
+            L.update(norm1=norm(hidden), norm2=norm(hidden), q_norm=norm(head_dim) if head_norms else None, k_norm=norm(head_dim) if head_norms else None)
+            L["k_cache"], L["v_cache"] = attention.new_cache(pages, page_size, self.kv_heads, head_dim)
+            self.layers.append(L)
+        self.norm = norm(hidden)
+        self.lm_head = synth.device_weight("Q6_K", vocab, hidden, gen)
+        self.cos, self.sin = attention.rope_tables(max_pages * page_size, head_dim, rope_base, rope_scaling)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        # tokens in the cache and block table of each request, and the stack of free pages: advanced on the GPU
+        self.ctx = torch.zeros(requests, **i32)
+        self.table = torch.full((requests, max_pages), -1, **i32)
+        self.free, self.free_count = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32), torch.full((1,), pages, **i32)
+        self.missing = torch.zeros(1, **i32)  # pages that the stack was short of, ever
+        self.one = torch.ones(requests, **i32)
+        self.workspace = attention.decode_workspace(self.q_heads, self.kv_heads, head_dim)
+        self.graph: Optional[DecodeGraph] = None
+
+    def _rms(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+        return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.eps) * w
+
+    def _forward(self, h: torch.Tensor, new: torch.Tensor, prompt: bool) -> torch.Tensor:
+        t = h.shape[0]
+        s = attention.paged_slots(self.ctx, new, self.table, self.page_size, self.free, self.free_count, t)
+        heads = lambda x: x.view(t, -1, self.head_dim)  # noqa: E731
+        for L in self.layers:
+            q, k, v = ops.rmsnorm_quant_matmul_batch(h, L["norm1"], self.eps, [L["q"], L["k"], L["v"]])
+            # a prompt's queries go to the tensor cores in the cache's type; a single token's stay as they are
+            q = attention.rope_append(heads(q), heads(k), heads(v), s.positions, self.cos, self.sin, L["k_cache"], L["v_cache"], s.slots,
+                                      q_weight=L["q_norm"], k_weight=L["k_norm"], eps=self.eps,
+                                      out_dtype=L["k_cache"].dtype if prompt else torch.float32)
+            over = dict(window=self.window, sinks=self.sinks)
+            if prompt:
+                a = attention.paged_prompt(q, s.cu_seqlens, L["k_cache"], L["v_cache"], self.table, s.seq_lens, **over)
+            else:
+                a = attention.paged_decode(q, L["k_cache"], L["v_cache"], self.table, s.seq_lens, workspace=self.workspace, **over)
+            h = h + ops.quant_matmul(a.view(t, -1), L["o"])
+            h = h + ops.quant_mlp(self._rms(h, L["norm2"]), L["gate"], L["up"], L["down"])
+        self.ctx.copy_(s.seq_lens)
+        self.free_count.copy_(s.left[:1])
+        self.missing.add_(s.left[1:])
+        if prompt:
+            h = h[(s.cu_seqlens[1:].long() - 1).clamp(min=0)]  # the newest token of each request
+        return ops.quant_matmul(self._rms(h, self.norm), self.lm_head)
+
+    def prompt(self, hidden: torch.Tensor, lengths: Sequence[int]) -> torch.Tensor:
+        """``lengths[b]`` new tokens of request b (0: none), their hidden states one request after the other [sum(lengths), hidden].
+        Logits [requests, vocab] of each request's newest token (of no meaning where there is none)."""
+        if len(lengths) != self.requests or hidden.shape[0] != sum(lengths):
+            raise ValueError(f"{sum(lengths)} hidden states for {self.requests} requests expected, got {hidden.shape[0]} for {len(lengths)}")
+        return self._forward(hidden, torch.tensor(lengths, dtype=torch.int32).to("cuda", non_blocking=True), True)
+
+    def step(self, hidden: torch.Tensor) -> torch.Tensor:
+        """One token of every request: hidden states [requests, hidden] to logits [requests, vocab]."""
+        return self._forward(hidden, self.one, False)
+
+    def capture(self) -> DecodeGraph:
+        """The step as a graph: ``replay(hidden=...)`` serves the next token of every request and returns ``{"logits": ...}``."""
+        x = torch.zeros(self.requests, self.hidden, device="cuda")
+        logits = torch.empty(self.requests, self.lm_head.shape[0], device="cuda")
+        kept = [t.clone() for t in (self.ctx, self.table, self.free_count, self.missing)]
+        g = DecodeGraph(lambda: logits.copy_(self.step(x)), {"hidden": x}, {"logits": logits}).capture()
+        # the warm-up served tokens that nobody sent: they are in places behind the newest tokens, which the next ones overwrite
+        for t, k in zip((self.ctx, self.table, self.free_count, self.missing), kept):
+            t.copy_(k)
+        self.graph = g
+        return g
+
+
+def main() -> None:
+    ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
+    ap.add_argument("--requests", type=int, default=8)
+    ap.add_argument("--prompt", type=int, default=1000, help="tokens of the longest prompt")
+    ap.add_argument("--steps", type=int, default=64)
+    ap.add_argument("--layers", type=int, default=LAYERS)
+    a = ap.parse_args()
+    lengths = [a.prompt - (a.prompt // 2) * b // max(1, a.requests) for b in range(a.requests)]
+    per = -(-(a.prompt + a.steps + 8) // 16)
+    stack = PagedStack(a.requests, pages=per * a.requests, max_pages=per, layers=a.layers)
+    x = torch.randn(sum(lengths), stack.hidden, device="cuda")
+    stack.prompt(x[: sum(min(n, 32) for n in lengths)], [min(n, 32) for n in lengths])  # the first calls load the kernels
+    stack.ctx.zero_()
+    stack.table.fill_(-1)
+    stack.free_count.fill_(per * a.requests)
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    stack.prompt(x, lengths)
+    torch.cuda.synchronize()
+    t1 = time.perf_counter()
+    g = stack.capture()
+    y = torch.randn(a.requests, stack.hidden, device="cuda")
+    g.replay(hidden=y)
+    torch.cuda.synchronize()
+    t2 = time.perf_counter()
+    for _ in range(a.steps):
+        g.replay(hidden=y)
+    torch.cuda.synchronize()
+    t3 = time.perf_counter()
+    ops.check_device_status()
+    print(f"prompts: {sum(lengths)} tokens in {(t1 - t0) * 1e3:.2f} ms; steps of {a.requests} requests: {(t3 - t2) / a.steps * 1e3:.3f} ms; "
+          f"missing pages: {int(stack.missing)}")
+
+
+if __name__ == "__main__":
+    main()

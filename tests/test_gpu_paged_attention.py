@@ -640,3 +640,110 @@ def test_rope_refusals(attention):
         attention.rope_append(*fine, out=torch.empty(3, 4, 32, device="cuda"))
     with pytest.raises(QuantError, match="output must be"):
         attention.rope_append(*fine, out_dtype=torch.float64)
+
+
+# ------------------------------------------------------------------------------- compiled entry points and the Python form
+
+
+def _outcome(call):
+    try:
+        r = call()
+    except Exception as e:
+        return type(e), str(e)
+    return [t.clone() for t in (r if isinstance(r, tuple) else (r,))]
+
+
+def test_both_forms_agree(attention, monkeypatch):
+    """The compiled entry points and the Python form: the same bits, the same refusals in the same words."""
+    from boostr_b200 import tensor
+
+    assert tensor.hostops().__name__ == "boostr_b200._hostops", "the compiled entry points are not built"
+    q, k, v, t, n = _fine(attention)
+    cu = _ints([0, 1, 2])
+    cos, sin = attention.rope_tables(40, 64)
+    kr, vr, pos, slots = q[:, :2], q[:, 2:], _ints([3, 4]), _ints([0, 17], torch.int64)
+    kc, vc = attention.new_cache(4, 16, 2, 64)
+    w = torch.rand(64, device="cuda")
+    out = torch.zeros_like(q)
+    wide = torch.cat([q, q], 2)[..., 32:96]
+    ws = attention.decode_workspace(4, 2, 64)
+    calls = {}
+    for name, f in (("decode", attention.paged_decode), ("prompt", lambda q, *a, **o: attention.paged_prompt(q, cu, *a, **o))):
+        c = lambda *a, f=f, **o: lambda: f(*a, **o)  # noqa: E731
+        calls.update({
+            f"{name}": c(q, k, v, t, n), f"{name} lse": c(q, k, v, t, n, return_lse=True), f"{name} f32 out": c(q, k, v, t, n, out_dtype=F32),
+            f"{name} out": c(q, k, v, t, n, out=out), f"{name} scale": c(q, k, v, t, n, scale=0.2, window=9, sinks=2), f"{name} int scale": c(q, k, v, t, n, scale=1),
+            f"{name} strided": c(wide, k, v, t, n), f"{name} f32": c(q.float(), k, v, t, n), f"{name} half": c(q.half(), k, v, t, n),
+            f"{name} lens": c(q, k, v, t, n[:1]), f"{name} long": c(q, k, v, t, n.long()), f"{name} window": c(q, k, v, t, n, window=-2),
+            f"{name} f64": c(q, k, v, t, n, out_dtype=torch.float64), f"{name} out shape": c(q, k, v, t, n, out=out[:1]),
+            f"{name} heads": c(q[:, :3], k, v, t, n), f"{name} empty": c(q[:0], k, v, t[:0], n[:0]) if name == "decode" else c(q[:0], k, v, t, n),
+        })
+    calls["decode workspace"] = lambda: attention.paged_decode(q, k, v, t, n, workspace=ws)
+    calls["decode small workspace"] = lambda: attention.paged_decode(q, k, v, t, n, workspace=ws[:4096])
+    calls["decode host workspace"] = lambda: attention.paged_decode(q, k, v, t, n, workspace=ws.cpu())
+    rope = lambda *a, **o: lambda: (attention.rope_append(*a, **o), kc.clone(), vc.clone())  # noqa: E731
+    calls.update({
+        "rope": rope(q, kr, vr, pos, cos, sin, kc, vc, slots), "rope norm": rope(q, kr, vr, pos, cos, sin, kc, vc, slots, w, w, 1),
+        "rope inter": rope(q, kr, vr, pos, cos, sin, kc, vc, slots, None, w, interleaved=True, out_dtype=F32),
+        "rope out": rope(q, kr, vr, pos, cos, sin, kc, vc, slots, out=torch.zeros_like(q)), "rope type": rope(q, kr.float(), vr, pos, cos, sin, kc, vc, slots),
+        "rope slots": rope(q, kr, vr, pos, cos, sin, kc, vc, slots.int()), "rope weight": rope(q, kr, vr, pos, cos, sin, kc, vc, slots, w[:32]),
+        "rope f64": rope(q, kr, vr, pos, cos, sin, kc, vc, slots, out_dtype=torch.float64), "rope table": rope(q, kr, vr, pos, cos[:3], sin, kc, vc, slots),
+    })
+    table = lambda: _ints([[7, -1], [8, -1]])  # noqa: E731
+    sl = lambda *a: lambda: tuple(attention.paged_slots(*a))  # noqa: E731
+    calls.update({"slots": sl(_ints([3, 16]), _ints([14, 2]), table(), 16, _ints([1, 2, 3]), _ints([3]), 18),
+                  "slots padded": sl(_ints([3, 16]), _ints([14, 2]), table(), 16, _ints([1, 2, 3]), _ints([1]), 20),
+                  "slots none": sl(_ints([3, 16]), _ints([0, 0]), table(), 16, _ints([1]), _ints([1]), 0),
+                  "slots page": sl(_ints([3, 16]), _ints([0, 0]), table(), 0, _ints([1]), _ints([1]), 0),
+                  "slots tokens": sl(_ints([3, 16]), _ints([0, 0]), table(), 16, _ints([1]), _ints([1]), -1),
+                  "slots lens": sl(_ints([3, 16]), _ints([0]), table(), 16, _ints([1]), _ints([1]), 1)})
+    compiled = {}
+    for name, call in calls.items():
+        kc.zero_(), vc.zero_()
+        compiled[name] = _outcome(call)
+    monkeypatch.setattr(tensor, "_hostops", tensor._PythonForms)
+    for name, call in calls.items():
+        kc.zero_(), vc.zero_()
+        a, b = compiled[name], _outcome(call)
+        assert type(a) is type(b), (name, a, b)
+        if isinstance(a, tuple):
+            assert a == b, name
+        else:
+            assert len(a) == len(b) and all(x.shape == y.shape and x.dtype == y.dtype and torch.equal(x, y) for x, y in zip(a, b)), name
+    refused = {n for n, r in compiled.items() if isinstance(r, tuple)}
+    assert refused == {x for x in calls if x.split(" ", 1)[-1] in ("half", "lens", "long", "window", "f64", "out shape", "heads", "small workspace", "host workspace",
+                                                                    "type", "slots", "weight", "table", "page", "tokens")} - {"slots"} | {"prompt f32"}, refused
+    ops.check_device_status()
+
+
+def test_scratch_of_threads_and_streams(attention):
+    """Threads on one stream and on their own: the joins of one call do not meet another's."""
+    import threading
+
+    g = _gen(15)
+    sets = []
+    for lens in ([9000], [700, 20000], [64] * 30):
+        k, v, t = make_cache(g, lens, 16, 2, 128, BF16)
+        q = _randn(g, len(lens), 16, 128, dtype=BF16)
+        sets.append((q, k, v, t, _ints(lens)))
+    want = [attention.paged_decode(*s) for s in sets]
+    torch.cuda.synchronize()
+    shared, errors = torch.cuda.Stream(), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(shared if i < 3 else torch.cuda.Stream()):
+                for r in range(40):
+                    j = (i + r) % len(sets)
+                    if not torch.equal(attention.paged_decode(*sets[j]), want[j]):
+                        raise AssertionError(f"thread {i}, pass {r}")
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    ops.check_device_status()
