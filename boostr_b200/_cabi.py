@@ -76,7 +76,8 @@ SIGNATURES = {
     "b200q_paged_decode": (c_int, [c_void_p, c_int, c_int64, c_int64, c_size_t, c_size_t, POINTER(PagedCache), c_void_p, c_int64, c_size_t,
                                    c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "b200q_paged_prompt": (c_int, [c_void_p, c_int, c_int64, c_int64, c_size_t, c_size_t, c_void_p, c_size_t, POINTER(PagedCache), c_void_p,
-                                   c_int64, c_size_t, c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_int, c_void_p, c_void_p]),
+                                   c_int64, c_size_t, c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "b200q_paged_prompt_workspace_bytes": (c_size_t, [c_size_t] * 8),
     "b200q_launch_count": (ctypes.c_ulonglong, []),
 }
 

@@ -248,7 +248,7 @@ def decode_workspace(q_heads: int, kv_heads: int, head_dim: int, device="cuda") 
 
 
 def _decode_workspace(nbytes: int, device) -> torch.Tensor:
-    """Scratch of ``paged_decode``, whose counters are zero between calls: one for each device and stream; a call that is being
+    """Scratch of the attentions, whose counters are zero between calls: one for each device and stream; a call that is being
     captured gets one of its own, zeroed by the graph."""
     nbytes = max(nbytes, 16)
     if torch.cuda.is_current_stream_capturing():
@@ -316,9 +316,12 @@ def paged_prompt(q: torch.Tensor, cu_seqlens: torch.Tensor, k_cache: torch.Tenso
     cu_seqlens = _ints(op, "cu_seqlens", cu_seqlens, (n + 1,))
     _same_device(op, q, cu_seqlens)
     lse = torch.empty(t, hq, dtype=torch.float32, device=q.device) if return_lse else None
+    L = _cabi.lib()
     with torch.cuda.device(q.device):
-        _cabi.check(_cabi.lib().b200q_paged_prompt(
+        need = L.b200q_paged_prompt_workspace_bytes(t, n, hq, k_cache.shape[2], q.shape[2], block_table.shape[1] * k_cache.shape[1], window, sinks) if n else 0
+        ws = _decode_workspace(need, q.device) if need else None
+        _cabi.check(L.b200q_paged_prompt(
             q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), t, hq, cu_seqlens.data_ptr(), n, cache, block_table.data_ptr(),
             block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), scale, window, sinks, out.data_ptr(), _DT[out.dtype],
-            lse.data_ptr() if return_lse else None, _stream()))
+            lse.data_ptr() if return_lse else None, ws.data_ptr() if need else None, ws.numel() if need else 0, _stream()))
     return (out, lse) if return_lse else out

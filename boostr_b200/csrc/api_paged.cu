@@ -9,7 +9,9 @@ namespace b200q {
 size_t slots_max_requests();
 cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st);
 cudaError_t launch_rope(const RopeParams& p, int dtype, bool interleaved, uint32_t run, cudaStream_t st);
-cudaError_t launch_prompt(const AttnParams& p, int sm_count, cudaStream_t st);
+size_t prompt_workspace_bytes(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hkv, uint32_t dim, uint64_t most, uint32_t window, uint32_t sinks,
+                              int sm_count);
+cudaError_t launch_prompt(const AttnParams& p, void* ws, int sm_count, cudaStream_t st);
 size_t decode_workspace_bytes(uint32_t group, uint32_t dim, int sm_count);
 cudaError_t launch_decode(const AttnParams& p, void* ws, int sm_count, cudaStream_t st);
 }  // namespace b200q
@@ -163,10 +165,19 @@ int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_stride, int64_t
     return finish(op, launch_decode(p, ws, api_sm_count(), static_cast<cudaStream_t>(stream)));
 }
 
+size_t b200q_paged_prompt_workspace_bytes(size_t tokens, size_t requests, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_len, size_t window,
+                                          size_t sinks) {
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads || q_heads > 65535 || head_dim == 0 || head_dim > 256 || tokens > MAX_INT || requests > MAX_INT ||
+        window > MAX_INT || sinks > MAX_INT || tokens == 0 || requests == 0)
+        return 0;
+    return prompt_workspace_bytes((uint32_t)tokens, (uint32_t)requests, (uint32_t)(q_heads / kv_heads), (uint32_t)kv_heads, (uint32_t)head_dim, max_len,
+                                  (uint32_t)window, (uint32_t)sinks, api_sm_count());
+}
+
 int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t tokens, size_t q_heads,
                        const int32_t* cu_seqlens, size_t requests, const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_row,
                        size_t width, const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out, int out_dtype, float* lse,
-                       void* stream) {
+                       void* ws, size_t ws_bytes, void* stream) {
     const char* op = "paged_prompt";
     if (tokens == 0 || requests == 0) return B200Q_OK;
     if (!cu_seqlens) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
@@ -176,7 +187,12 @@ int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t
                            scale, window, sinks, out, out_dtype, lse))
         return rc;
     p.cu = cu_seqlens;
-    return finish(op, launch_prompt(p, api_sm_count(), static_cast<cudaStream_t>(stream)));
+    if (ws) {
+        const size_t need = prompt_workspace_bytes(p.rows, p.requests, p.group, p.hkv, p.dim, (uint64_t)p.width * p.page.d, p.window, p.sinks, api_sm_count());
+        if (ws_bytes < need || !aligned(ws, 16))
+            return api_fail(B200Q_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes is too small or not 16-byte aligned, need %zu", op, ws_bytes, need);
+    }
+    return finish(op, launch_prompt(p, ws, api_sm_count(), static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -458,15 +458,15 @@ at::ScalarType out_type(PyObject* given, long code, const at::Tensor& q) {
     return given != Py_None && THPVariable_CheckExact(given) ? THPVariable_Unpack(given).scalar_type() : q.scalar_type();
 }
 
-// Scratch of paged_decode, apart from the other operators' because its counters are zero between calls; like theirs, one for
+// Scratch of the attentions, apart from the other operators' because its counters are zero between calls; like theirs, one for
 // each (device, stream), and one of its own for a call that is being captured, zeroed by the graph.
 auto& g_counters = *new std::map<std::pair<int, cudaStream_t>, std::unique_ptr<Scratch>>;
 template <typename F>
 int with_counters(c10::Device dev, size_t need, const at::Tensor* given, F&& call) {
     const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    if (given) {
+    if (given || !need) {
         NoGil nogil;
-        return call(given->data_ptr(), (size_t)given->numel(), st);
+        return call(given ? given->data_ptr() : nullptr, given ? (size_t)given->numel() : 0, st);
     }
     if (capturing(st)) {
         const at::Tensor buf = empty({(int64_t)need}, at::kByte, dev);
@@ -658,11 +658,13 @@ PyObject* paged_prompt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if (!attn_of(args, a) || a.q->scalar_type() == at::kFloat) return not_served();
         const at::Tensor* cu = vector_of(args[11], at::kInt, d, a.lens->size(0) + 1);
         if (!cu) return not_served();
-        const int rc = with_scratch(d, 0, [&](void*, size_t, cudaStream_t st) {
+        const size_t need = b200q_paged_prompt_workspace_bytes((size_t)a.q->size(0), (size_t)a.lens->size(0), (size_t)a.q->size(1), a.c.kv_heads, a.c.head_dim,
+                                                               (size_t)a.table->size(1) * a.c.page_size, a.window, a.sinks);
+        const int rc = with_counters(d, need, nullptr, [&](void* ws, size_t bytes, cudaStream_t st) {
             return b200q_paged_prompt(a.q->data_ptr(), dtype_code(a.q->scalar_type()), a.q->stride(0), a.q->stride(1), (size_t)a.q->size(0),
                                       (size_t)a.q->size(1), cu->data_ptr<int>(), (size_t)a.lens->size(0), &a.c, a.table->data_ptr<int>(), a.table->stride(0),
                                       (size_t)a.table->size(1), a.lens->data_ptr<int>(), a.scale, a.window, a.sinks, a.out.data_ptr(), a.odt,
-                                      a.lse.defined() ? a.lse.data_ptr<float>() : nullptr, st);
+                                      a.lse.defined() ? a.lse.data_ptr<float>() : nullptr, ws, bytes, st);
         });
         return attn_result(rc, a);
     });

@@ -30,6 +30,9 @@ struct PromptPlan {
     uint32_t idesc_s, idesc_o;
     uint32_t ksteps;       // of 16 elements of a head
     uint32_t nq;           // query tiles of a CTA: 1 or 2
+    uint32_t splits;       // CTAs that share the keys of the same query tiles, at most
+    float* part;           // of each CTA and query tile, where there are several: O [DP / 4][128][4], {m, l} [128]
+    uint32_t* counters;    // [grid / splits] zero between calls
     uint32_t rows;         // tokens of a TMA box of the cache: they lie in one page (0: no TMA)
 };
 
@@ -42,6 +45,11 @@ constexpr float PR_BIAS = F16 ? 9.f : 0.f;  // f16 weights are kept 2^9 times th
 // Of every eight pairs of weights, this many are computed by exp2_poly: the special-function unit takes 8 cycles for a warp's 32
 // exponentials, the cubic's instructions a good half of that.
 constexpr int PR_POLY = 2;
+
+// Where CTAs are few (a chunk of some tokens at the end of a long context), several share the keys of the same rows, in runs of no fewer
+// tiles than this; the one that finishes last adds their sums up in order.  (32 heads of
+// 128 over 8, us without and with: 1 row of 8000 keys 89.3, 20.6; 30 rows of 30000 keys 317, 73.7; 128 rows of 8000 keys 91.7, 64.0.)
+constexpr uint32_t PR_MIN_TILES = 4, PR_MAX_SPLITS = 16;
 
 constexpr int PR_THREADS = 512;
 constexpr int PR_LOADERS = 128;
@@ -237,7 +245,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                    bar_done = bar_v + 8 * DEPTH;
     volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 256);
     volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + Sh::OFF_BAR + 260);
-    __shared__ uint32_t s_scan[PR_THREADS / 32], s_find[5];
+    __shared__ uint32_t s_scan[PR_THREADS / 32], s_find[5], s_last;
 
     if (threadIdx.x == 0) {
         mbar_init(bar_q, 1);
@@ -257,7 +265,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
     PromptWork w;
     bool idle;
     {
-        const uint32_t per = p.hkv * d.chunks, pair_rev = blockIdx.x / per, hc = blockIdx.x - pair_rev * per, step = d.nq * d.tokens;
+        const uint32_t unit = blockIdx.x / d.splits, per = p.hkv * d.chunks, pair_rev = unit / per, hc = unit - pair_rev * per, step = d.nq * d.tokens;
         w.head = hc / d.chunks;
         w.chunk = hc - w.head * d.chunks;
         const uint32_t n = (p.requests + PR_THREADS - 1) / PR_THREADS;
@@ -319,9 +327,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         w.pos0 = (int64_t)s_find[4] - (int64_t)last_row + w.row0;
         const int64_t last = w.pos0 + w.rows;  // one behind the last row's position
         // whole boxes: some keys more, which the rows' own limits hide
-        const uint32_t unit = d.rows ? d.rows : 1;
-        w.from = p.window && w.pos0 + 1 > (int64_t)p.window ? (uint32_t)(w.pos0 + 1 - p.window) / unit * unit : 0;
-        w.sinks = min((p.sinks + unit - 1) / unit * unit, w.from);
+        const uint32_t box = d.rows ? d.rows : 1;
+        w.from = p.window && w.pos0 + 1 > (int64_t)p.window ? (uint32_t)(w.pos0 + 1 - p.window) / box * box : 0;
+        w.sinks = min((p.sinks + box - 1) / box * box, w.from);
         w.keys = last > 0 && w.rows ? w.sinks + (uint32_t)last - w.from : 0;
     }
     const uint32_t tmem = *tmem_holder;
@@ -331,7 +339,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
         const int64_t end = w.pos0 + min(w.rows, (t + 1) * d.tokens);
         return end > 0 && w.keys ? (w.sinks + (uint32_t)end - w.from + NK - 1) / NK : 0u;
     };
-    const uint32_t n0 = tiles_of(0), nt = tiles_of(nq - 1);
+    // this CTA's tiles of keys: [tile0, tile0 + nt), and the first query tile's of them
+    const uint32_t all = tiles_of(nq - 1), shares = max(1u, min(d.splits, all / PR_MIN_TILES)), share = blockIdx.x % d.splits;
+    const bool none = share >= shares;
+    const uint32_t tile0 = none ? 0 : share * all / shares, nt = none ? 0 : (share + 1) * all / shares - tile0;
+    const uint32_t n0 = min(nt, max(tiles_of(0), tile0) - tile0);
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -443,13 +455,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             };
             // Whole tiles come by TMA where boxes fit into pages: a lane finds the page of a box and issues it.  A warp takes 200 cycles for each
             // box, so all four share every tile (one warp a tile: the keys came late).
-            const uint32_t whole = d.rows ? w.keys / NK : 0, lw = tid >> 5;  // tiles by TMA
+            const uint32_t whole = d.rows ? min(w.keys / NK, tile0 + nt) - tile0 : 0, lw = tid >> 5;  // tiles by TMA
             if (whole) {
                 const uint32_t boxes = NK / d.rows * blocks, own = (boxes + 3 - lw) / 4, box = lw + 4 * lane, g = box / blocks, b = box - g * blocks;
                 auto tile = [&](uint32_t kv, uint32_t i) {
                     uint32_t page = 0, tok = 0;
                     if (lane < own) {
-                        const uint32_t v = i * NK + g * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
+                        const uint32_t v = (tile0 + i) * NK + g * d.rows, key = v < w.sinks ? v : v - w.sinks + w.from;
                         if (!attn_page(p, w.b, key, page, tok)) page = p.pages;
                     }
                     room(kv, i);
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             };
             for (uint32_t j = whole; j < nt; ++j) {  // to the end in any case: the loaders meet at barriers
                 uint64_t* at = rows + j % 3 * 256;   // a third one is written while the slowest thread reads the first
-                const uint32_t v = j * NK + tid;
+                const uint32_t v = (tile0 + j) * NK + tid;
                 uint64_t ka = 0, va = 0;
                 if (tid < NK && v < w.keys) {
                     const uint32_t key = v < w.sinks ? v : v - w.sinks + w.from;
@@ -559,16 +571,16 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[c][i] ^= 0x80000000u;
-            if (j >= open_end) {
-                const int end = (int)min(hi, 0x40000000u) - (int)(j * NK);
+            if (tile0 + j >= open_end) {
+                const int end = (int)min(hi, 0x40000000u) - (int)((tile0 + j) * NK);
 #pragma unroll
                 for (int c = 0; c < NK / 16; ++c)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (16 * c + i >= end) s[c][i] = 0xFF800000u;
             }
-            if (j >= cut_from && j < cut_to) {  // [a, a + n) is hidden
-                const int a = (int)p.sinks - (int)(j * NK);
+            if (tile0 + j >= cut_from && tile0 + j < cut_to) {  // [a, a + n) is hidden
+                const int a = (int)p.sinks - (int)((tile0 + j) * NK);
                 const uint32_t n = lo > p.sinks ? lo - p.sinks : 0;
 #pragma unroll
                 for (int c = 0; c < NK / 16; ++c)
@@ -648,17 +660,114 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             }
             tc_after();
         }
-        if (t < nq && ok) {
+        const int64_t row = (int64_t)(w.row0 + tok) * p.hq + w.head * p.group + h;
+        float odd = 0.f;  // not zero: some element is not finite
+        const bool split = shares > 1 && !none;
+        bool write = t < nq && ok && !none;
+        if (split && t < nq) {
+            // ---- the rows' sums to scratch (in a CTA that gave up, too: the count has to come out even), [element / 4][row][4]
+            constexpr size_t PART = 128 * DP + 256;
+            const uint32_t rows = min(w.rows - min(w.rows, t * d.tokens), d.tokens) * d.heads;  // of the tile
+            float* part = d.part + ((size_t)blockIdx.x * d.nq + t) * PART;
+            if (mine)
+#pragma unroll 1
+                for (uint32_t c = 0; c < p.dim; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16_async(o_at + c, o);
+                    tmem_ld_wait();
+                    if (r < rows)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            *reinterpret_cast<uint4*>(part + ((c / 4 + u) * 128 + r) * 4) = make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                }
+            *reinterpret_cast<float2*>(part + 128 * DP + 2 * r) = make_float2(mine ? m : -INFINITY, mine ? l : 0.f);
+            named_bar_sync(2, 128 * nq);
+            if (threadIdx.x == 0) {
+                __threadfence();  // the CTA's sums, which the barrier has shown to this thread, before the count
+                const uint32_t done = atomicAdd(d.counters + blockIdx.x / d.splits, 1u) == shares - 1 ? 1u : 0u;
+                __threadfence();
+                if (done) d.counters[blockIdx.x / d.splits] = 0;  // for the next call
+                s_last = done;
+            }
+            named_bar_sync(2, 128 * nq);
+            write = write && s_last;
+            if (s_last) {
+                // ---- the last one adds up all CTAs' sums, in their order
+                const float* parts = d.part + ((size_t)(blockIdx.x - share) * d.nq + t) * PART;
+                const size_t next = d.nq * PART;
+                // [split][row] factors, then the rows' inverse sums, then whether a row came out not finite; the ring is at rest
+                float* factors = reinterpret_cast<float*>(smem + Sh::OFF_K) + t * ((PR_MAX_SPLITS + 2) * 128);
+                float top = -INFINITY;
+                for (uint32_t i = 0; i < shares; ++i) top = fmaxf(top, __ldcg(parts + i * next + 128 * DP + 2 * r));
+                l = 0.f;
+                for (uint32_t i = 0; i < shares; ++i) {
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + i * next + 128 * DP + 2 * r));
+                    // a NaN maximum (fmaxf passes it over) makes its factor and the sums NaN
+                    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+                    factors[i * 128 + r] = f;
+                    l = fmaf(ml.y, f, l);
+                }
+                m = top;
+                factors[PR_MAX_SPLITS * 128 + r] = l == 0.f ? 0.f : 1.f / l;
+                factors[(PR_MAX_SPLITS + 1) * 128 + r] = 0.f;
+                named_bar_sync(2, 128 * nq);
+                // four elements by four splits on their way at a time
+                const uint32_t items = rows * (p.dim / 4);
+                for (uint32_t e0 = r; e0 < items; e0 += 4 * 128) {
+                    uint32_t c4[4], of[4];
+                    float4 a[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t e = min(e0 + 128 * u, items - 1);
+                        c4[u] = e / rows, of[u] = e - c4[u] * rows;
+                        a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll 1
+                    for (uint32_t k0 = 0; k0 < shares; k0 += 4) {
+                        float4 x[4][4];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                x[k][u] = __ldcg(reinterpret_cast<const float4*>(parts + min(k0 + k, shares - 1) * next + (c4[u] * 128 + of[u]) * 4));
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const float f = k0 + k < shares ? factors[(k0 + k) * 128 + of[u]] : 0.f;
+                                if (f != 0.f)  // what has no weight may not be there
+                                    a[u].x = fmaf(x[k][u].x, f, a[u].x), a[u].y = fmaf(x[k][u].y, f, a[u].y), a[u].z = fmaf(x[k][u].z, f, a[u].z),
+                                    a[u].w = fmaf(x[k][u].w, f, a[u].w);
+                            }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        if (e0 + 128 * u >= items) break;
+                        const float inv = factors[PR_MAX_SPLITS * 128 + of[u]];
+                        const float y[4] = {a[u].x * inv, a[u].y * inv, a[u].z * inv, a[u].w * inv};
+                        // 0 x is not 0 where x is not finite
+                        if (!(y[0] * 0.f + y[1] * 0.f + y[2] * 0.f + y[3] * 0.f == 0.f)) factors[(PR_MAX_SPLITS + 1) * 128 + of[u]] = 1.f;
+                        const uint32_t to_tok = t * d.tokens + of[u] / d.heads, to_h = w.chunk * d.heads + of[u] % d.heads;
+                        if (to_h < p.group) {
+                            const int64_t to = ((int64_t)(w.row0 + to_tok) * p.hq + w.head * p.group + to_h) * p.dim + 4 * c4[u];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) store_f32(p.out, to + i, p.out_dtype, y[i]);
+                        }
+                    }
+                }
+                named_bar_sync(2, 128 * nq);
+                odd = factors[(PR_MAX_SPLITS + 1) * 128 + r];
+            }
+        }
+        if (write) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int64_t row = (int64_t)(w.row0 + tok) * p.hq + w.head * p.group + h;
-            float odd = 0.f;  // not zero: some element is not finite
             // Results of the cache's type go through the rows of the query tile in shared memory, which nothing reads any more, so that a
             // warp writes whole rows: 16-byte chunks, swapped by row against bank conflicts.  Small loops: code that runs once for a block
             // costs more by its fetching than by its running.
             uint8_t* stage = smem + Sh::OFF_Q + t * Sh::Q_TILE + (warp & 3) * (32 * DP * 2);
             const bool staged = p.out_dtype == (F16 ? DT_F16 : DT_BF16);
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < p.dim; c0 += 64) {
+            for (uint32_t c0 = split ? p.dim : 0; c0 < p.dim; c0 += 64) {
                 uint32_t o[64 / 16][16];
 #pragma unroll
                 for (int u = 0; u < 64 / 16; ++u)
@@ -684,7 +793,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
                 }
             }
             __syncwarp();
-            if (staged) {
+            if (staged && !split) {
                 constexpr uint32_t CPR = DP / 8;
                 const uint32_t all_live = __ballot_sync(0xFFFFFFFFu, live), chunk = lane % CPR;
 #pragma unroll 1
@@ -762,27 +871,55 @@ cudaError_t prompt_go(const AttnParams& p, PromptPlan& d, uint32_t grid, cudaStr
     return launch_pdl(prompt_kernel<DP, F16>, dim3(grid), dim3(PR_THREADS), PromptShape<DP>::SMEM, st, p, d, q, k, v);
 }
 
-}  // namespace
-
-cudaError_t launch_prompt(const AttnParams& p, int sm_count, cudaStream_t st) {
-    PromptPlan d;
-    d.heads = p.group < 128 ? p.group : 128;
-    d.chunks = (p.group + d.heads - 1) / d.heads;
+// Of a call: its plan without the operands.  `most`: tokens that a request can have.
+PromptPlan prompt_plan(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hkv, uint32_t dim, uint64_t most, uint32_t window, uint32_t sinks, int sm_count,
+                       uint64_t& units) {
+    PromptPlan d = {};
+    d.heads = group < 128 ? group : 128;
+    d.chunks = (group + d.heads - 1) / d.heads;
     d.tokens = 128 / d.heads;
-    const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, nk = dp == 256 ? PromptShape<256>::NK : dp == 128 ? PromptShape<128>::NK : PromptShape<64>::NK;
-    d.ksteps = (p.dim + 15) / 16;
-    const uint32_t type = p.f16 ? 0u : 1u, common = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);  // f32 sums, M = 128
-    d.idesc_s = common | ((nk >> 3) << 17);
-    d.idesc_o = common | (1u << 16) | ((d.ksteps * 16 >> 3) << 17);  // B: rows of tokens
-    // pairs of tiles there can be: whole ones, and one more at the end of each request
+    const uint32_t dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, nk = dp == 256 ? PromptShape<256>::NK : dp == 128 ? PromptShape<128>::NK : PromptShape<64>::NK;
+    d.ksteps = (dim + 15) / 16;
+    // tiles, or pairs of them, that there can be: whole ones, and one more at the end of each request
     auto blocks = [&](uint32_t nq) {
-        const uint64_t n = (uint64_t)p.rows / (nq * d.tokens) + p.requests;
-        return (n > p.rows ? (uint64_t)p.rows : n) * p.hkv * d.chunks;
+        const uint64_t n = (uint64_t)rows / (nq * d.tokens) + requests;
+        return (n > rows ? (uint64_t)rows : n) * hkv * d.chunks;
     };
     // Two query tiles a CTA read the keys once and alternate on the tensor core; where that leaves half of the SMs without a CTA, one is
     // faster (512 tokens, 32 heads of 128 over 8: 17.2 us and 15.5).
     d.nq = dp == 256 || 2 * blocks(2) <= (uint64_t)sm_count ? 1 : 2;
-    const uint64_t grid = blocks(d.nq);
+    units = blocks(d.nq);
+    if (window) most = most < (uint64_t)window + sinks + d.nq * d.tokens + 256 ? most : (uint64_t)window + sinks + d.nq * d.tokens + 256;
+    const uint64_t fit = units ? (uint64_t)sm_count / units : 1, worth = most / ((uint64_t)nk * PR_MIN_TILES);
+    uint64_t splits = fit < worth ? fit : worth;
+    d.splits = splits < 1 ? 1 : splits > PR_MAX_SPLITS ? PR_MAX_SPLITS : (uint32_t)splits;
+    return d;
+}
+
+constexpr size_t PR_COUNTER_BYTES = 4096;
+
+}  // namespace
+
+size_t prompt_workspace_bytes(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hkv, uint32_t dim, uint64_t most, uint32_t window, uint32_t sinks,
+                              int sm_count) {
+    uint64_t units;
+    const PromptPlan d = prompt_plan(rows, requests, group, hkv, dim, most, window, sinks, sm_count, units);
+    if (d.splits == 1) return 0;
+    const size_t dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+    return PR_COUNTER_BYTES + units * d.splits * d.nq * (128 * dp + 256) * sizeof(float);
+}
+
+cudaError_t launch_prompt(const AttnParams& p, void* ws, int sm_count, cudaStream_t st) {
+    uint64_t units;
+    PromptPlan d = prompt_plan(p.rows, p.requests, p.group, p.hkv, p.dim, (uint64_t)p.width * p.page.d, p.window, p.sinks, sm_count, units);
+    if (!ws) d.splits = 1;
+    d.counters = static_cast<uint32_t*>(ws);
+    d.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + PR_COUNTER_BYTES);
+    const uint32_t dp = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, nk = dp == 256 ? PromptShape<256>::NK : dp == 128 ? PromptShape<128>::NK : PromptShape<64>::NK;
+    const uint32_t type = p.f16 ? 0u : 1u, common = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);  // f32 sums, M = 128
+    d.idesc_s = common | ((nk >> 3) << 17);
+    d.idesc_o = common | (1u << 16) | ((d.ksteps * 16 >> 3) << 17);  // B: rows of tokens
+    const uint64_t grid = units * d.splits;
     if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
     if (dp == 64) return p.f16 ? prompt_go<64, true>(p, d, (uint32_t)grid, st) : prompt_go<64, false>(p, d, (uint32_t)grid, st);
     if (dp == 128) return p.f16 ? prompt_go<128, true>(p, d, (uint32_t)grid, st) : prompt_go<128, false>(p, d, (uint32_t)grid, st);

@@ -387,11 +387,15 @@ B200Q_API int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_strid
  * last tokens of request b (all of which are in the cache), and each sees what a decode step at its position would.
  * q of the cache's type.  Rows of a request that has more rows than tokens see nothing and are zero (lse -inf), and so are
  * rows behind cu_seqlens[requests].
+ * ws: NULL, or b200q_paged_prompt_workspace_bytes bytes for max_len = width * page_size (0: none needed) on the terms of
+ * b200q_paged_decode's; with it few rows that see many keys are split over the keys.
  */
+B200Q_API size_t b200q_paged_prompt_workspace_bytes(size_t tokens, size_t requests, size_t q_heads, size_t kv_heads, size_t head_dim, size_t max_len,
+                                                    size_t window, size_t sinks);
 B200Q_API int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, size_t tokens, size_t q_heads,
                                  const int32_t* cu_seqlens, size_t requests, const b200q_paged_cache* cache, const int32_t* block_table,
                                  int64_t table_row, size_t width, const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out,
-                                 int out_dtype, float* lse, void* stream);
+                                 int out_dtype, float* lse, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -131,5 +131,7 @@ extern "C" {
     pub fn b200q_paged_prompt(q: *const c_void, q_dtype: c_int, q_row_stride: i64, q_head_stride: i64, tokens: usize, q_heads: usize,
                               cu_seqlens: *const i32, requests: usize, cache: *const b200q_paged_cache, block_table: *const i32, table_row: i64,
                               width: usize, seq_lens: *const i32, scale: f32, window: usize, sinks: usize, out: *mut c_void, out_dtype: c_int,
-                              lse: *mut f32, stream: *mut c_void) -> c_int;
+                              lse: *mut f32, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn b200q_paged_prompt_workspace_bytes(tokens: usize, requests: usize, q_heads: usize, kv_heads: usize, head_dim: usize, max_len: usize,
+                                              window: usize, sinks: usize) -> usize;
 }

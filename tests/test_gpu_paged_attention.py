@@ -274,6 +274,12 @@ PROMPT = [
     ([(0, 700)], 128, 8, 4, 128, 130, 0, BF16, BF16, "tokens", 0),
     ([(0, 1500)], 16, 4, 4, 128, 0, 0, BF16, BF16, "tokens", 0),
     ([(6000, 700)], 16, 4, 1, 128, 0, 0, BF16, BF16, "tokens", 0),
+    # few rows over many keys: the keys are split and joined
+    ([(20000, 3)], 16, 32, 8, 128, 0, 0, BF16, BF16, "tokens", 0),
+    ([(30000, 1), (9000, 40), (0, 5), (100, 0)], 64, 8, 2, 64, 0, 0, F16, F32, "heads", 2),
+    ([(7000, 70)], 16, 4, 1, 256, 0, 0, BF16, BF16, "tokens", 0),
+    ([(9000, 20), (400, 30)], 7, 6, 1, 80, 0, 0, F16, F16, "joint", 0),
+    ([(50000, 9)], 32, 16, 2, 128, 3000, 20, BF16, BF16, "heads", 0),
 ]
 
 

@@ -87,4 +87,4 @@ def test_cabi_refusals():
     assert L.b200q_paged_slots(p, p, 0, p, 3, 3, 16, p, 9, p, p, p, p, p, 4, p, None) == _cabi.ERR_BAD_SHAPE
     assert L.b200q_paged_slots(p, p, 2, p, 3, 3, 0, p, 9, p, p, p, p, p, 4, p, None) == _cabi.ERR_BAD_SHAPE
     assert L.b200q_paged_slots(p, None, 2, p, 3, 3, 16, p, 9, p, p, p, p, p, 4, p, None) == _cabi.ERR_INVALID_ARG
-    assert L.b200q_paged_prompt(p, _cabi.DT_F32, 256, 64, 2, 4, p, 1, cache(), p, 3, 3, p, 1.0, 0, 0, p, 0, None, None) == _cabi.ERR_UNSUPPORTED_DTYPE
+    assert L.b200q_paged_prompt(p, _cabi.DT_F32, 256, 64, 2, 4, p, 1, cache(), p, 3, 3, p, 1.0, 0, 0, p, 0, None, None, 0, None) == _cabi.ERR_UNSUPPORTED_DTYPE
