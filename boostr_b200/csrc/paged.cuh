@@ -138,6 +138,13 @@ __device__ __forceinline__ uint32_t request_of(const int32_t* cu, uint32_t reque
     return lo;
 }
 
+// Counts one more and returns the count before; what this thread has seen written is visible to whoever reads a later count.
+__device__ __forceinline__ uint32_t count_up(uint32_t* counter) {
+    uint32_t r;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(r) : "l"(counter) : "memory");
+    return r;
+}
+
 // ------------------------------------------------------------------------------------------- copies and matrix instructions
 
 // 16 bytes global -> shared, asynchronously; `bytes` (0 or 16) of them are read, the rest is filled with zeros

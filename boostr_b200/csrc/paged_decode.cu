@@ -528,9 +528,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecodeShape<DP, NT, F16, SPLIT>::
                     const uint32_t first = (uint32_t)(((g0 + 1) * active - 1) / total), last = (uint32_t)(((g1 + 1) * active - 1) / total);
                     uint32_t done = 0;
                     if (threadIdx.x == 0) {
-                        __threadfence();  // the CTA's parts, which the barrier has shown to this thread, before the count
-                        done = atomicAdd(d.counters + first, 1u) == last - first ? 1u : 0u;
-                        __threadfence();
+                        // the CTA's parts, which the barrier has shown to this thread, before the count; the others' behind it
+                        done = count_up(d.counters + first) == last - first ? 1u : 0u;
                         if (done) d.counters[first] = 0;  // for the next call
                         s_last = done;
                     }

@@ -683,9 +683,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) prompt_kernel(const AttnParams 
             *reinterpret_cast<float2*>(part + 128 * DP + 2 * r) = make_float2(mine ? m : -INFINITY, mine ? l : 0.f);
             named_bar_sync(2, 128 * nq);
             if (threadIdx.x == 0) {
-                __threadfence();  // the CTA's sums, which the barrier has shown to this thread, before the count
-                const uint32_t done = atomicAdd(d.counters + blockIdx.x / d.splits, 1u) == shares - 1 ? 1u : 0u;
-                __threadfence();
+                // the CTA's sums, which the barrier has shown to this thread, before the count; the others' behind it
+                const uint32_t done = count_up(d.counters + blockIdx.x / d.splits) == shares - 1 ? 1u : 0u;
                 if (done) d.counters[blockIdx.x / d.splits] = 0;  // for the next call
                 s_last = done;
             }
