@@ -92,7 +92,7 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, uint32_t lane) {
 // Adds up the parts of CTAs first .. last of elements dim .. dim + 3 of a head, in that order.
 template <int HEADS, int DP>
 __device__ __forceinline__ void join_parts(const float* parts, uint32_t first, uint32_t last, uint32_t head, uint32_t dim, float4& a, float& mx, float& sum) {
-    constexpr int AT_ONCE = 16, PART = HEADS * (DP + 2);
+    constexpr int AT_ONCE = 8, PART = HEADS * (DP + 2);
     a = make_float4(0.f, 0.f, 0.f, 0.f);
     mx = -INFINITY, sum = 0.f;
     for (uint32_t c0 = first; c0 <= last; c0 += AT_ONCE) {
