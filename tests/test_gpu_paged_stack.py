@@ -59,9 +59,12 @@ def test_graph_advances_by_itself():
 
 
 def test_pool_that_runs_dry():
-    """Requests beyond the last page: their tokens are not kept, the others go on."""
+    """Requests beyond the last page: their tokens are not kept, the attention meets the hole and says so."""
+    from boostr_b200._cabi import B200QError
     from boostr_b200.paged_stack import PagedStack
 
     s = PagedStack(2, pages=3, **{**SMALL, "max_pages": 4})
     s.prompt(torch.randn(50, 512, device="cuda"), [20, 30])
     assert int(s.missing) == 1 and int(s.free_count) == 0
+    with pytest.raises(B200QError, match="out of range"):
+        ops.check_device_status()
