@@ -223,10 +223,8 @@ def _attn_args(op, q, k_cache, v_cache, block_table, seq_lens, scale, window, si
     _table(op, block_table, seq_lens.shape[0])
     _same_device(op, q, k_cache, v_cache, block_table, seq_lens)
     unit = 16 // q.element_size()
-    if (q.stride(2) != 1 and d > 1) or q.stride(0) % unit or q.stride(1) % unit:
-        q = q.contiguous()
-    if q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
+    if q.stride(2) != 1 or any(q.stride(i) % unit or (q.stride(i) == 0 and q.shape[i] > 1) for i in (0, 1)) or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)  # contiguous() keeps the odd stride of a single row
     out_dtype = out_dtype or (out.dtype if out is not None else q.dtype)
     if out_dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise QuantError(f"{op}: output must be F32, BF16 or F16, got {out_dtype}")

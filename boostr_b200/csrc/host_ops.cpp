@@ -601,7 +601,7 @@ bool attn_of(PyObject* const* args, Attn& a) {
     const int qdt = dtype_code(q.scalar_type());
     const int64_t unit = qdt == B200Q_F32 ? 4 : 8;
     if (q.size(2) != (int64_t)a.c.head_dim || q.size(1) % (int64_t)a.c.kv_heads || (qdt != B200Q_F32 && qdt != a.c.dtype) || q.stride(0) % unit ||
-        q.stride(1) % unit || (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15))
+        q.stride(1) % unit || (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) || (q.size(0) > 1 && q.stride(0) == 0) || (q.size(1) > 1 && q.stride(1) == 0))
         return false;
     a.scale = args[5] == Py_None ? (float)std::pow((double)a.c.head_dim, -0.5) : (float)PyFloat_AsDouble(args[5]);
     const long code = PyLong_AsLong(args[8]);

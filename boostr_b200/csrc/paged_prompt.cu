@@ -847,7 +847,9 @@ bool query_map(CUtensorMap* map, const AttnParams& p, const PromptPlan& d) {
     const EncodeTiledFn encode = encode_tiled();
     if (!encode) return false;
     const cuuint64_t dims[3] = {p.dim, p.hq, p.rows};
-    const cuuint64_t strides[2] = {(cuuint64_t)p.q_head * 2, (cuuint64_t)p.q_row * 2};
+    // the stride of a dimension of one is never taken, but has to be one
+    const cuuint64_t head = p.hq == 1 ? (cuuint64_t)p.dim * 2 : (cuuint64_t)p.q_head * 2;
+    const cuuint64_t strides[2] = {head, p.rows == 1 ? head * p.hq : (cuuint64_t)p.q_row * 2};
     const cuuint32_t box[3] = {64, d.heads, d.tokens}, one[3] = {1, 1, 1};
     return encode(map, p.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p.q), dims, strides, box, one,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -196,6 +196,19 @@ def test_decode_strided_queries_and_given_output(attention):
     q = rows[:, : 16 * 64].view(2, 16, 64)
     want = attention.paged_decode(q.contiguous(), k, v, table, _ints(lens))
     assert torch.equal(attention.paged_decode(q, k, v, table, _ints(lens)), want)
+    one = q[:1, :1].expand(2, 16, 64)  # one head for all: copied
+    assert torch.equal(attention.paged_decode(one, k, v, table, _ints(lens)), attention.paged_decode(one.contiguous(), k, v, table, _ints(lens)))
+    cu = _ints([0, 1, 2])
+    assert torch.equal(attention.paged_prompt(one, cu, k, v, table, _ints(lens)), attention.paged_prompt(one.contiguous(), cu, k, v, table, _ints(lens)))
+    flat = q[0].reshape(-1).as_strided((1, 16, 64), (0, 64, 1))  # one row whose stride says nothing
+    assert torch.equal(attention.paged_prompt(flat, cu[:2], k, v, table[:1], _ints(lens[:1])), attention.paged_prompt(q[:1], cu[:2], k, v, table[:1], _ints(lens[:1])))
+    single = rows.new_zeros(1, 16 * 64 + 5)[:, : 16 * 64].view(1, 16, 64)  # one row of an odd stride
+    single.copy_(q[:1])
+    assert torch.equal(attention.paged_decode(single, k, v, table[:1], _ints(lens[:1])), want[:1])
+    assert torch.equal(attention.paged_prompt(single, cu[:2], k, v, table[:1], _ints(lens[:1])), attention.paged_prompt(q[:1].contiguous(), cu[:2], k, v, table[:1], _ints(lens[:1])))
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)  # heads before tokens in memory
+    assert torch.equal(attention.paged_decode(turned, k, v, table, _ints(lens)), want)
+    assert torch.equal(attention.paged_prompt(turned, cu, k, v, table, _ints(lens)), attention.paged_prompt(q, cu, k, v, table, _ints(lens)))
     odd = _randn(g, 2, 16, 65, dtype=BF16)
     odd[..., 1:] = q
     assert torch.equal(attention.paged_decode(odd[..., 1:], k, v, table, _ints(lens)), want)  # unaligned: copied
