@@ -1,22 +1,27 @@
 // Causal attention of the new tokens of prompts over a paged cache, on the 5th-generation tensor cores.
 //
-// A CTA owns two tiles of 128 query rows (one for heads over 128 wide).  A row is one query head of one token; all query heads
-// that share a key-value head stand next to one another, so a tile is 128 / group tokens and every key and value is read once for
-// all of them.  The keys that any row of the CTA sees (the sinks, then everything from the first row's window to the last
-// row's position) are numbered through without a gap and visited in tiles of 128.
+// A CTA owns two tiles of 128 query rows (one for heads over 128 wide, or where CTAs are few).  A row is one query head of one token; all
+// query heads that share a key-value head stand next to one another, so a tile is 128 / group tokens and every key and value is read
+// once for all of them.  The keys that any row of the CTA sees (the sinks, then everything from the first row's window to the last row's
+// position) are numbered through without a gap and visited in tiles of NK.
 //
 //   scores   S = Q K^T: tcgen05.mma, Q and K in shared memory, S (f32) in tensor memory;
-//   softmax  one thread a row: reads its 128 scores, takes the weights P = 2^(s - m) against a maximum that follows the row only
+//   softmax  one thread a row: reads its scores, takes the weights P = 2^(s - m) against a maximum that follows the row only
 //            when a score exceeds it by 2^SLACK (then the row's sums are rescaled in tensor memory), writes P as 16-bit
 //            elements back to tensor memory;
 //   values   O += P V: P from tensor memory, V as it lies in shared memory (token rows, so the MMA reads it "MN-major").
 //
-// Warps 0-3 and 4-7 are the softmax of the two tiles, and while one works on its scores the tensor core has the other's products;
-// warps 8-11 bring the rows of the pages into a ring of swizzled tiles: by TMA, a box for each run of up to 128 tokens inside
-// a page, or, where pages are no multiple of 8 tokens and in the last tile, by 16-byte asynchronous copies, which leave zeros where
-// there is no visible key (so nothing that lies in unused places reaches a sum); warp 12 issues the MMAs.
-// Bound: 4 flops for each visible pair and element on the tensor cores, and one exponential for each pair.
+// Warps 0-3 and 4-7 are the softmax of the two tiles; warps 8-11 bring the rows of the pages into rings of swizzled tiles: by TMA, a
+// box for each run of tokens inside a page, or, where pages are no multiple of 8 tokens and in the last tile, by 16-byte asynchronous
+// copies, which leave zeros where there is no visible key (so nothing that lies in unused places reaches a sum); a thread of warp 12 and one of
+// warp 13 issue the products of a tile each.
 // A product of a zero weight and a value that is not finite is not zero: rows that come out not finite are computed once more, key by key.
+//
+// Bound: 4 flops for each visible pair and element on the tensor cores, and one exponential for each pair.  Measured (32 heads of 128 over
+// 8, bf16): a prompt of 8192 tokens 553 us, 993 TFLOP/s at the part's power limit (1670 MHz; 477 us, 1150 TFLOP/s, before it is reached);
+// 0.61 of cuBLAS's burst rate, 0.73 of its sustained one.  Tensor pipe busy 47 % of the cycles, special functions 36 %, issue slots 47 %:
+// the two softmax groups run in step, and of a step of 2600 cycles 1500 are the products'.  Tiles of 64 to 128 keys, other shares of the
+// cubic, and a shift between the groups change the time by 2 % at most.
 #include "paged.cuh"
 #include "tcgen05_i8.cuh"
 #include "tmap.cuh"
