@@ -17,7 +17,7 @@ its calls, which comes from the graph's own memory pool and lives as long as the
 The fused row-parallel exchange carries its epoch in device memory, so a captured step that contains it
 replays without any host-side argument.  ``DeviceScalars`` are the two stream-updated int32 values of the
 reference (``seq_len_k``, ``write_pos``); the quantized linears do not read them, attention kernels of a
-host model would.
+host model would.  (The attention of this library keeps its lengths in tensors of its own: ``attention.paged_slots``.)
 """
 from __future__ import annotations
 

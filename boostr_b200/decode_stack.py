@@ -2,7 +2,7 @@
 composes them (src/model/llama/model_tp.rs:321-359, block_tp.rs:72-102, 299-304): q/k/v as one batched
 column-parallel projection, o row-parallel, gate/up through ``quant_swiglu``, down row-parallel, and a
 column-parallel lm_head whose logits are gathered.  Attention, normalisation and the residual stream are
-not part of the quantized-linear path and are left out: o_proj consumes the q projection, and every layer
+not part of the quantized-linear path and are left out here (``paged_stack`` has them): o_proj consumes the q projection, and every layer
 starts again from the step input so magnitudes stay finite.
 
 Used by ``bench.py`` (Llama-3-8B shapes, Q4_K_M mix) and by the graph-replay tests (small shapes).

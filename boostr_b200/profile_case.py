@@ -4,10 +4,14 @@
     python -m boostr_b200.profile_case --op swiglu  --fmt Q4_K --m 1 --n 14336 --k 4096 --copies 4 --iters 8
     python -m boostr_b200.profile_case --op qkv     --m 1 --k 4096 --copies 8 --iters 16
     python -m boostr_b200.profile_case --op dequant --fmt Q6_K --n 16384 --k 4096 --dtype bf16
+    python -m boostr_b200.profile_case --op paged_decode --m 1 --tokens 131072
+    python -m boostr_b200.profile_case --op paged_prompt --m 4096 --copies 1
+    python -m boostr_b200.profile_case --op rope_append  --m 8192 --dtype bf16
 
 The weights are random packed blocks generated on the device (scales drawn as in the synthetic
 benchmark inputs); `--copies` distinct weights are used in rotation so that launches stream from HBM
-instead of the 126 MB L2.  Without a profiler attached it prints the average device time per call,
+instead of the 126 MB L2.  The attention operators take a Llama-3-8B-shaped layer (32 query heads over 8 of 128, bf16 pages of 16
+tokens): ``--m`` requests of ``--tokens`` tokens (paged_decode), or ``--m`` new tokens of one request (paged_prompt, rope_append).  Without a profiler attached it prints the average device time per call,
 measured with CUDA events around `--iters` back-to-back calls after three warm-up calls.
 """
 from __future__ import annotations
@@ -19,13 +23,43 @@ import sys
 from .synth import device_weight  # noqa: E402
 
 
+def _attention_case(a, gen):
+    import torch
+
+    from . import attention
+
+    hq, hk, d, page = 32, 8, 128, 16
+    requests, length = (a.m, a.tokens) if a.op == "paged_decode" else (1, a.m)
+    per = -(-length // page)
+    table = torch.randperm(requests * per, device="cuda", generator=gen).to(torch.int32).view(requests, per)
+    caches = [tuple(torch.randn(requests * per, page, hk, d, device="cuda", generator=gen).bfloat16() for _ in range(2)) for _ in range(a.copies)]
+    lens = torch.full((requests,), length, dtype=torch.int32, device="cuda")
+    kv = 2 * requests * length * hk * d * 2
+    if a.op == "paged_decode":
+        q = torch.randn(requests, hq, d, device="cuda", generator=gen).to(torch.float32 if a.dtype == "f32" else torch.bfloat16)
+        return lambda j: attention.paged_decode(q, *caches[j], table, lens), kv, 0
+    q = torch.randn(length, hq, d, device="cuda", generator=gen).bfloat16()
+    if a.op == "paged_prompt":
+        cu = torch.tensor([0, length], dtype=torch.int32, device="cuda")
+        return lambda j: attention.paged_prompt(q, cu, *caches[j], table, lens), kv + 4 * q.numel(), 2 * length * (length + 1) * hq * d
+    act = torch.float32 if a.dtype == "f32" else torch.bfloat16
+    rows = torch.randn(length, (hq + 2 * hk) * d, device="cuda", generator=gen).to(act)
+    q, k, v = (x.view(length, -1, d) for x in rows.split([hq * d, hk * d, hk * d], 1))
+    cos, sin = attention.rope_tables(length, d)
+    pos, w = torch.arange(length, device="cuda", dtype=torch.int32), torch.ones(d, device="cuda")
+    slots = torch.randperm(per * page, device="cuda", generator=gen)[:length].contiguous()
+    nbytes = rows.numel() * rows.element_size() + q.numel() * q.element_size() + kv
+    return lambda j: attention.rope_append(q, k, v, pos, cos, sin, *caches[j], slots, w, w), nbytes, 0
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("--op", choices=["matmul", "swiglu", "qkv", "dequant"], default="matmul")
+    ap.add_argument("--op", choices=["matmul", "swiglu", "qkv", "dequant", "paged_decode", "paged_prompt", "rope_append"], default="matmul")
     ap.add_argument("--fmt", default="Q4_K")
     ap.add_argument("--m", type=int, default=1)
     ap.add_argument("--n", type=int, default=14336)
     ap.add_argument("--k", type=int, default=4096)
+    ap.add_argument("--tokens", type=int, default=4096)
     ap.add_argument("--copies", type=int, default=4)
     ap.add_argument("--iters", type=int, default=8)
     ap.add_argument("--dtype", choices=["f32", "bf16"], default="f32", help="activation dtype (dequant: output dtype)")
@@ -49,6 +83,8 @@ def main(argv=None) -> int:
 
         def run(j):
             QuantLinear.forward_batch(sets[j], act, outs=outs)
+    elif a.op in ("paged_decode", "paged_prompt", "rope_append"):
+        run, nbytes, flops = _attention_case(a, gen)
     elif a.op == "dequant":
         ws = [device_weight(a.fmt, a.n, a.k, gen) for _ in range(a.copies)]
         esz = 4 if a.dtype == "f32" else 2
@@ -81,7 +117,8 @@ def main(argv=None) -> int:
     torch.cuda.synchronize()
     ops.check_device_status()
     us = e0.elapsed_time(e1) * 1000.0 / a.iters
-    msg = f"{a.op} fmt={a.fmt} M={a.m} N={a.n} K={a.k} {a.dtype}: {us:.2f} us/call (stream-ordered, not graphed), {nbytes / us / 1e3:.1f} GB/s"
+    shape = f"M={a.m} tokens={a.tokens}" if a.op in ("paged_decode", "paged_prompt", "rope_append") else f"fmt={a.fmt} M={a.m} N={a.n} K={a.k}"
+    msg = f"{a.op} {shape} {a.dtype}: {us:.2f} us/call (stream-ordered, not graphed), {nbytes / us / 1e3:.1f} GB/s"
     if flops and a.m >= 64:
         msg += f", {flops / us / 1e6:.1f} TFLOP/s"
     print(msg)
