@@ -166,7 +166,7 @@ __device__ __forceinline__ void store_n(void* base, int64_t i0, const float (&x)
 // A row is one head of one token.  G neighbouring lanes share it; a lane owns U units of two runs of C elements: the two
 // that a rotation turns into one another (i and i + rot / 2 of the half layout; 2 C neighbours of the interleaved one), so
 // no element crosses lanes, or 2 C neighbours behind the rotated part.  Bound: HBM, each element is read and written once; what it
-// is short of that goes to instructions (2/3 of the issue slots: conversions, the sum of squares, addresses).  8192 tokens of 48 heads of
+// is short of that goes to instructions (61 % of the issue slots: conversions, the sum of squares, addresses).  8192 tokens of 48 heads of
 // 128, bf16 with norms: 47.5 us, 4.3 TB/s.  Two to four rows a lane, with all loads first or one after the other with the angles kept, were slower
 // (60 to 83 us: fewer threads fit).
 template <typename T, int C, int G, int U, bool INTERLEAVED>
