@@ -55,11 +55,16 @@ int fill_attn(const char* op, AttnParams& p, const b200q_paged_cache* c, const v
         return api_fail(B200Q_ERR_BAD_SHAPE, "%s: %zu query heads do not share %zu key-value heads evenly", op, q_heads, c->kv_heads);
     if (rows > MAX_INT || requests > MAX_INT || width > MAX_INT || window > MAX_INT || sinks > MAX_INT || rows * q_heads > MAX_INT)
         return api_fail(B200Q_ERR_BAD_SHAPE, "%s: dimension too large (rows=%zu requests=%zu table width=%zu)", op, rows, requests, width);
-    if (!q || !table || !lens || !out) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
+    if (!q || (requests && (!table || !lens)) || !out) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
     const int64_t unit = 16 / (int64_t)type_bytes(q_dtype);
     if (!aligned(q, 16) || q_row % unit || q_head % unit || q_row < 0 || q_head < 0)
         return api_fail(B200Q_ERR_INVALID_ARG, "%s: query heads must be 16-byte aligned", op);
     if (!aligned(out, 16)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: output pointer must be 16-byte aligned", op);
+    // a row's queries are read by several CTAs, and again where its sums are not finite
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+    const size_t q_bytes = ((rows - 1) * (size_t)q_row + (q_heads - 1) * (size_t)q_head + c->head_dim) * type_bytes(q_dtype);
+    if (o0 < q0 + q_bytes && q0 < o0 + rows * q_heads * c->head_dim * type_bytes(out_dtype))
+        return api_fail(B200Q_ERR_INVALID_ARG, "%s: the output must not overlap the queries", op);
     if (width == 0 || table_row < 0) return api_fail(B200Q_ERR_BAD_SHAPE, "%s: empty block table", op);
     if (!std::isfinite(scale)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: scale must be finite", op);
     p.q = q, p.q_row = q_row, p.q_head = q_head, p.q_dtype = q_dtype;
@@ -179,7 +184,7 @@ int b200q_paged_prompt(const void* q, int q_dtype, int64_t q_row_stride, int64_t
                        size_t width, const int32_t* seq_lens, float scale, size_t window, size_t sinks, void* out, int out_dtype, float* lse,
                        void* ws, size_t ws_bytes, void* stream) {
     const char* op = "paged_prompt";
-    if (tokens == 0 || requests == 0) return B200Q_OK;
+    if (tokens == 0) return B200Q_OK;
     if (!cu_seqlens) return api_fail(B200Q_ERR_INVALID_ARG, "%s: null pointer", op);
     if (q_dtype == DT_F32) return api_fail(B200Q_ERR_UNSUPPORTED_DTYPE, "%s: queries must have the cache's type", op);
     AttnParams p = {};

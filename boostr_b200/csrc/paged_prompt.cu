@@ -888,7 +888,7 @@ PromptPlan prompt_plan(uint32_t rows, uint32_t requests, uint32_t group, uint32_
     d.ksteps = (dim + 15) / 16;
     // tiles, or pairs of them, that there can be: whole ones, and one more at the end of each request
     auto blocks = [&](uint32_t nq) {
-        const uint64_t n = (uint64_t)rows / (nq * d.tokens) + requests;
+        const uint64_t n = (uint64_t)rows / (nq * d.tokens) + (requests ? requests : 1);  // no request: somebody writes the zeros
         return (n > rows ? (uint64_t)rows : n) * hkv * d.chunks;
     };
     // Two query tiles a CTA read the keys once and alternate on the tensor core; where that leaves half of the SMs without a CTA, one is

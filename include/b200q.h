@@ -369,7 +369,7 @@ B200Q_API int b200q_rope_append(const b200q_heads* q, const b200q_heads* k, cons
  * Attention of one new token per request, the last of its seq_lens[b] tokens (which is in the cache): out[b, h] =
  * sum_j softmax_j(scale q[b, h] . k[j]) v[j] over the keys that it sees: all, or with window > 0 the last `window` and the
  * first `sinks`.  A request of length 0 gives zeros (lse -inf).  q: F32 or the cache's type; out [requests, q_heads,
- * head_dim] F32, BF16 or F16; lse [requests, q_heads] (natural logarithm of the sum of exponentials) or NULL.
+ * head_dim] F32, BF16 or F16, not overlapping q; lse [requests, q_heads] (natural logarithm of the sum of exponentials) or NULL.
  * Scores, softmax and sums are f32; with F32 queries the products keep the queries' and weights' upper 16 bits or more
  * (queries of an F16 cache below 65504).
  * ws: b200q_paged_decode_workspace_bytes bytes (0: bad arguments), 16-byte aligned, whose first B200Q_PAGED_COUNTER_BYTES are zero before its first
@@ -386,7 +386,7 @@ B200Q_API int b200q_paged_decode(const void* q, int q_dtype, int64_t q_row_strid
  * Causal attention of the new tokens of prompts, whole or in chunks: rows cu_seqlens[b] .. cu_seqlens[b + 1] of q are the
  * last tokens of request b (all of which are in the cache), and each sees what a decode step at its position would.
  * q of the cache's type.  Rows of a request that has more rows than tokens see nothing and are zero (lse -inf), and so are
- * rows behind cu_seqlens[requests].
+ * rows behind cu_seqlens[requests] (all rows where there is no request).
  * ws: NULL, or b200q_paged_prompt_workspace_bytes bytes for max_len = width * page_size (0: none needed) on the terms of
  * b200q_paged_decode's; with it few rows that see many keys are split over the keys.
  */

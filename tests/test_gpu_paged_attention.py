@@ -188,6 +188,30 @@ def test_decode_infinite_scores_and_values(attention):
     check(out, None, reference(q, _ints([399]), 0, ref, v, table, 400, d ** -0.5, 0, 0)[:3] + (torch.full((1, 8), 500.0, device="cuda"),), q, F16, F16, False)
 
 
+def test_output_over_the_queries_is_refused(attention):
+    g = _gen(7)
+    k, v, table = make_cache(g, [40, 9], 16, 2, 64, BF16)
+    q = _randn(g, 2, 8, 64, dtype=BF16)
+    pool = torch.empty(3, 8, 64, dtype=BF16, device="cuda")
+    pool[:2] = q
+    for out in (pool[:2], pool[1:]):
+        with pytest.raises(_cabi.B200QError, match="must not overlap"):
+            attention.paged_decode(pool[:2], k, v, table, _ints([40, 9]), out=out)
+        with pytest.raises(_cabi.B200QError, match="must not overlap"):
+            attention.paged_prompt(pool[:2], _ints([0, 1, 2]), k, v, table, _ints([40, 9]), out=out)
+    want = attention.paged_decode(q[:1], k, v, table[:1], _ints([40]))
+    assert torch.equal(attention.paged_decode(pool[:1], k, v, table[:1], _ints([40]), out=pool[1:2]), want)  # next to them
+
+
+@pytest.mark.parametrize("rows", [1, 5, 700])
+def test_prompt_of_no_request_is_zero(attention, rows):
+    g = _gen(8)
+    k, v, table = make_cache(g, [40], 16, 2, 64, BF16)
+    out = torch.ones(rows, 8, 64, dtype=BF16, device="cuda")
+    _, lse = attention.paged_prompt(_randn(g, rows, 8, 64, dtype=BF16), _ints([0]), k, v, table[:0], _ints([]), out=out, return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+
+
 def test_decode_strided_queries_and_given_output(attention):
     g = _gen(6)
     lens = [333, 20]
