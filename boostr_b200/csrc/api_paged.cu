@@ -60,13 +60,13 @@ int fill_attn(const char* op, AttnParams& p, const b200q_paged_cache* c, const v
     if (!aligned(q, 16) || q_row % unit || q_head % unit || q_row < 0 || q_head < 0)
         return api_fail(B200Q_ERR_INVALID_ARG, "%s: query heads must be 16-byte aligned", op);
     if (!aligned(out, 16)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: output pointer must be 16-byte aligned", op);
+    if (width == 0 || table_row < 0) return api_fail(B200Q_ERR_BAD_SHAPE, "%s: empty block table", op);
+    if (!std::isfinite(scale)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: scale must be finite", op);
     // a row's queries are read by several CTAs, and again where its sums are not finite
     const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
     const size_t q_bytes = ((rows - 1) * (size_t)q_row + (q_heads - 1) * (size_t)q_head + c->head_dim) * type_bytes(q_dtype);
     if (o0 < q0 + q_bytes && q0 < o0 + rows * q_heads * c->head_dim * type_bytes(out_dtype))
         return api_fail(B200Q_ERR_INVALID_ARG, "%s: the output must not overlap the queries", op);
-    if (width == 0 || table_row < 0) return api_fail(B200Q_ERR_BAD_SHAPE, "%s: empty block table", op);
-    if (!std::isfinite(scale)) return api_fail(B200Q_ERR_INVALID_ARG, "%s: scale must be finite", op);
     p.q = q, p.q_row = q_row, p.q_head = q_head, p.q_dtype = q_dtype;
     p.k = static_cast<const uint8_t*>(c->k), p.v = static_cast<const uint8_t*>(c->v);
     p.k_page = c->k_strides[0], p.k_tok = c->k_strides[1], p.k_head = c->k_strides[2];
