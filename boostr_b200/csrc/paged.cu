@@ -134,7 +134,7 @@ cudaError_t launch_slots(const SlotsParams& p, int sm_count, cudaStream_t st) {
 
 namespace {
 
-constexpr int RP_THREADS = 256;
+constexpr int RP_THREADS = 128;
 
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Pack {
@@ -166,11 +166,12 @@ __device__ __forceinline__ void store_n(void* base, int64_t i0, const float (&x)
 // A row is one head of one token.  G neighbouring lanes share it; a lane owns U units of two runs of C elements: the two
 // that a rotation turns into one another (i and i + rot / 2 of the half layout; 2 C neighbours of the interleaved one), so
 // no element crosses lanes, or 2 C neighbours behind the rotated part.  Bound: HBM, each element is read and written once; what it
-// is short of that goes to instructions (61 % of the issue slots: conversions, the sum of squares, addresses).  8192 tokens of 48 heads of
-// 128, bf16 with norms: 47.5 us, 4.3 TB/s.  Two to four rows a lane, with all loads first or one after the other with the angles kept, were slower
-// (60 to 83 us: fewer threads fit).
+// is short of that goes to instructions (70 % of the issue slots: conversions, the sum of squares, addresses) and to the one load that each
+// warp waits for.  8192 tokens of 48 heads of 128, bf16 with norms: 43.8 us, 4.6 TB/s, by 12 blocks of 128 threads of 40 registers an SM (five blocks
+// of 256 threads of 48: 47.8; six of 40: 45.5; seven, or blocks of 64: 52 and more).  Two to four rows a lane, with all loads first or one
+// after the other with the angles kept, were slower (60 to 83 us: fewer threads fit).
 template <typename T, int C, int G, int U, bool INTERLEAVED>
-__global__ void __launch_bounds__(RP_THREADS, C == 8 ? 5 : 1) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(RP_THREADS, C == 8 ? 12 : 1) rope_kernel(const RopeParams p) {
     grid_dep_wait();
     grid_dep_launch();
     const uint32_t row = blockIdx.x * (RP_THREADS / G) + threadIdx.x / G, g = threadIdx.x % G;
